@@ -92,6 +92,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_gemm_k", &grouped_gemm_k);
   m.def("grouped_gemm_fp8_m", &grouped_gemm_fp8_m);
   m.def("sf_tiles", &sf_tiles);
+  m.def("grouped_gemm_fp8_block", &grouped_gemm_fp8_block);
+  m.def("quant_fp8_weight", &quant_fp8_weight);
+  m.def("router_gate", &router_gate);
+  m.def("router_gate_bwd", &router_gate_bwd);
   m.def("wait_probe", &wait_probe);
   m.def("fence_cost", &fence_cost);
   m.def("nvl_bw", &nvl_bw, "raw NVLink engine bandwidth probe (all-to-all pattern)");

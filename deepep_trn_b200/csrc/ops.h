@@ -126,6 +126,19 @@ void grouped_gemm_fp8_m(const at::Tensor& A, const at::Tensor& sa, const at::Ten
 void grouped_gemm_k(const at::Tensor& A, const at::Tensor& B, const at::Tensor& offsets, at::Tensor C,
                     at::Tensor error, int64_t num_sms, double timeout_s, bool tok_major);
 
+// gemm_block.cu
+void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
+                            const OptTensor& offsets, const OptTensor& counts, const OptTensor& C, const OptTensor& H,
+                            const OptTensor& Hs, int64_t epilogue, const at::Tensor& error, int64_t num_sms,
+                            double timeout_s, bool b_kn);
+
+// gate.cu
+std::tuple<at::Tensor, at::Tensor> router_gate(const at::Tensor& logits, int64_t topk, bool sigmoid,
+                                               const OptTensor& bias, int64_t num_groups, int64_t topk_groups,
+                                               bool top2, bool renorm, double scale);
+at::Tensor router_gate_bwd(const at::Tensor& logits, const at::Tensor& idx, const at::Tensor& dw, bool sigmoid,
+                           bool renorm, double scale);
+
 // moe.cu
 void router_topk(const at::Tensor& logits, int64_t topk, at::Tensor idx, at::Tensor w);
 void router_topk_bwd(const at::Tensor& idx, const at::Tensor& w, const at::Tensor& dw, at::Tensor dlogits);
@@ -142,5 +155,6 @@ void transpose(const at::Tensor& in, at::Tensor out);
 // quant.cu
 void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_scale);
 void dequant_fp8(const at::Tensor& q, const at::Tensor& scales, at::Tensor out);
+std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w);
 
 }  // namespace b200ep

@@ -3,8 +3,10 @@
 ``grouped_gemm``       C[seg_e] = A[seg_e] @ B[e]^T      A [rows, K], B [G, N, K]   (forward)
                        C[seg_e] = A[seg_e] @ B[e]        A [rows, K], B [G, K, N]   (``b_layout='kn'``: dX)
 ``grouped_gemm_wgrad`` C[e] = A[seg_e]^T @ B[seg_e]      A [tok, M], B [tok, N]     (dW)
-``grouped_gemm_fp8``   C[seg_e] = A[seg_e] @ B[e]^T      e4m3 A, B with 1x128 power-of-two scales
                        C[e] = A[:, seg_e] @ B[:, seg_e]^T A [M, tok], B [N, tok]    (``layout='mk'``)
+``grouped_gemm_fp8``   C[seg_e] = A[seg_e] @ B[e]^T      e4m3 A, B with 1x128 power-of-two scales
+``grouped_gemm_fp8_block``  the same with arbitrary fp32 scales (A 1x128, B 128x128), either layout of B,
+                       segments of any length or one slab per group, and SwiGLU + e4m3 output in the epilogue
 
 Transposed operands are read in place by the tensor cores (MN-major shared-memory
 descriptors), never materialised.
@@ -18,7 +20,8 @@ from __future__ import annotations
 
 import torch
 
-from ._ext import load
+from ..utils.codec import FP8_BLOCK, dequantize_fp8_128x128, quantize_fp8_1x128, quantize_fp8_128x128
+from ._ext import available, load
 
 _errors: dict = {}
 EPILOGUES = {'bf16': 0, 'f32': 1, 'swiglu': 2}
@@ -78,7 +81,6 @@ def quantize_fp8_blocks(w: torch.Tensor):
     """e4m3 copy of ``w`` [.., K] with one power-of-two fp32 scale per (row, 128-channel block):
     the operand format of ``grouped_gemm_fp8`` (the tensor cores apply the scales as UE8M0
     exponents, so they must be powers of two)."""
-    from ..utils.codec import quantize_fp8_1x128
     q, sc = quantize_fp8_1x128(w, round_scale=True)
     return q.contiguous(), sc.contiguous()
 
@@ -116,6 +118,91 @@ def grouped_gemm_fp8(A, sa, B, sb, offsets, out=None, epilogue: str = 'bf16', h_
     load().grouped_gemm_fp8_m(a8, sa, b8, sb, offsets, c, None, EPILOGUES[epilogue], _err(A.device), num_sms,
                               timeout_s)
     return c
+
+
+FP8_BLOCK_EPILOGUES = {'bf16': 0, 'f32': 1, 'swiglu': 2}
+
+
+def quantize_fp8_weight(w: torch.Tensor):
+    """e4m3 copy of ``w`` [N, K] or [G, N, K] (fp32, bf16 or fp16) with one fp32 scale per
+    128 x 128 block (the last blocks of a side may be short): ``(q, scales [.., ceil(N/128),
+    ceil(K/128)])`` with ``w ~= q * scale``, ``scale = max(amax, 1e-4) / 448``. The operand format
+    of ``grouped_gemm_fp8_block``; a transposed product reads the same pair (``b_layout='kn'``)."""
+    if not w.is_cuda:
+        if available():
+            load().quant_fp8_weight(w)   # the argument checks
+        return quantize_fp8_128x128(w)
+    q, sc = load().quant_fp8_weight(w)
+    return q.view(torch.float8_e4m3fn), sc
+
+
+def grouped_gemm_fp8_block(A, sa, B, sb, offsets=None, counts=None, out=None, epilogue: str = 'bf16',
+                           b_layout: str = 'nk', h_out=None, h_scales=None, save_preact: bool = False,
+                           num_sms: int = 0, timeout_s: float = 10.0):
+    """Grouped fp8 GEMM with arbitrary fp32 scales, one per 128 channels:
+    ``C[rows of g] = (A * sa)[rows of g] @ (B[g] * sb[g])^T``.
+
+    A and B are e4m3. ``sa`` has one fp32 scale per row of A and 128 channels (``quantize_fp8``, or
+    what an fp8 dispatch delivers), ``sb`` [G, ceil(N/128), ceil(K/128)] one per 128 x 128 block of
+    B [G, N, K] (``quantize_fp8_weight``). ``b_layout='kn'`` takes B as [G, K, N] with sb
+    [G, ceil(K/128), ceil(N/128)], read in place: with a forward weight and its scales that is the
+    gradient of the product's input. K is a multiple of 16, N of 8 (``'kn'``: 16).
+
+    Rows: A [rows, K] with ``offsets`` [G + 1] int64 (nondecreasing; any lengths, also zero), or
+    A [G, cap, K], one slab per group (a low-latency dispatch's layout, strided slabs included).
+    ``counts`` [G] int32, with either, gives the rows in use from the start of each group. Rows
+    that belong to no group, or lie behind a count, are not written: a new output holds anything there.
+
+    Sums are fp32 (each block of 128 products is scaled and added in fp32). ``epilogue='bf16'`` and
+    ``'f32'`` return C. ``'swiglu'`` reads each 256 columns as [128 gate | 128 up]
+    (``interleave_gate_up``) and returns ``(h, h_scales, pre)``: ``h = silu(gate) * up`` in e4m3 with
+    fp32 1x128 scales, the operand of the next product, and the bf16 pre-activation with
+    ``save_preact`` (else None). ``out``, ``h_out``, ``h_scales`` receive C / pre, h and its scales.
+    """
+    if epilogue not in FP8_BLOCK_EPILOGUES:
+        raise ValueError(f'unknown epilogue {epilogue!r}; expected one of {tuple(FP8_BLOCK_EPILOGUES)}')
+    if b_layout not in ('nk', 'kn'):
+        raise ValueError(f"unknown b_layout {b_layout!r}; expected 'nk' or 'kn'")
+    kn = b_layout == 'kn'
+    N = B.shape[2 if kn else 1]
+    lead = A.shape[:-1]
+    h = hs = None
+    if epilogue == 'swiglu':
+        h = h_out if h_out is not None else torch.empty(*lead, N // 2, dtype=torch.float8_e4m3fn, device=A.device)
+        hs = h_scales if h_scales is not None else torch.empty(*lead, N // 256, dtype=torch.float32, device=A.device)
+        c = (out if out is not None else torch.empty(*lead, N, dtype=torch.bfloat16, device=A.device)) \
+            if save_preact else None
+    else:
+        dtype = torch.float32 if epilogue == 'f32' else torch.bfloat16
+        c = out if out is not None else torch.empty(*lead, N, dtype=dtype, device=A.device)
+    if A.is_cuda or available():   # on CPU tensors: the argument checks
+        load().grouped_gemm_fp8_block(A, sa, B, sb, offsets, counts, c, h, hs, FP8_BLOCK_EPILOGUES[epilogue],
+                                      _err(A.device), num_sms, timeout_s, kn)
+    if not A.is_cuda:
+        _grouped_gemm_fp8_block_cpu(A, sa, B, sb, offsets, counts, c, h, hs, kn)
+    return c if epilogue != 'swiglu' else (h, hs, c)
+
+
+def _grouped_gemm_fp8_block_cpu(A, sa, B, sb, offsets, counts, c, h, hs, kn):
+    """The torch definition (fp32), into c and / or h and hs."""
+    Bf = dequantize_fp8_128x128(B.view(torch.float8_e4m3fn), sb)
+    Bf = Bf if kn else Bf.transpose(1, 2)
+    Af = A.view(torch.float8_e4m3fn).float() * sa.repeat_interleave(FP8_BLOCK, -1)[..., :A.shape[-1]]
+    for g in range(B.shape[0]):
+        rows = A.shape[-2]
+        begin, end = (0, rows) if A.dim() == 3 else (min(max(int(offsets[g]), 0), rows), min(int(offsets[g + 1]), rows))
+        if counts is not None:
+            end = min(end, begin + max(int(counts[g]), 0))
+        end = max(end, begin)
+        at = (g, slice(begin, end)) if A.dim() == 3 else (slice(begin, end),)
+        y = Af[at] @ Bf[g]
+        if c is not None:
+            c[at] = y.to(c.dtype)
+        if h is not None:
+            gate, up = deinterleave(y)
+            q, sc = quantize_fp8_1x128(torch.nn.functional.silu(gate) * up)
+            h.view(torch.uint8)[at] = q.view(torch.uint8)
+            hs[at] = sc
 
 
 def interleave_gate_up(w_gate: torch.Tensor, w_up: torch.Tensor, block: int = 128) -> torch.Tensor:

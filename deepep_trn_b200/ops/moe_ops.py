@@ -1,12 +1,12 @@
-"""Wrappers of the MoE-layer kernels (router top-k, permute/unpermute, SwiGLU backward,
+"""Wrappers of the MoE-layer kernels (router top-k, gate, permute/unpermute, SwiGLU backward,
 transpose). CUDA tensors run the sm_100a kernels; CPU tensors run the torch definitions
 below, which double as the numerics oracle in the tests."""
 from __future__ import annotations
 
 import torch
 
-from ..utils.testing import router_topk_reference
-from ._ext import load
+from ..utils.testing import router_gate_bwd_reference, router_gate_reference, router_topk_reference
+from ._ext import available, load
 
 ALIGN = 128  # expert segments of the permuted layout start at multiples of this
 
@@ -39,6 +39,52 @@ def router_topk_bwd(idx: torch.Tensor, w: torch.Tensor, dw: torch.Tensor, num_ex
     out = torch.empty(w.shape[0], num_experts, dtype=torch.float32, device=w.device)
     load().router_topk_bwd(idx.contiguous(), w.float().contiguous(), dw.float().contiguous(), out)
     return out
+
+
+def router_gate(logits: torch.Tensor, k: int, scoring: str = 'sigmoid', bias: torch.Tensor | None = None,
+                num_groups: int = 1, topk_groups: int = 1, group_score: str = 'top2', renormalize: bool = True,
+                scale: float = 1.0):
+    """Expert selection from router logits [T, E] (fp32, bf16 or fp16): ``(ids int64, weights fp32) [T, k]``.
+
+    Scores are ``sigmoid(logits)`` or ``softmax(logits)`` over the experts (``scoring``). ``bias``
+    [E] fp32 is added for the selection only (a load-balancing bias). With ``num_groups`` > 1 the
+    experts compete inside the best ``topk_groups`` groups of E / num_groups consecutive experts,
+    ranked by the sum of their two largest selection values (``group_score='top2'``) or by the
+    largest (``'max'``). The k largest are taken in order, ties to the lower id; where 32-bit
+    scores are too close to tell, fp64 ones decide. Weights are the scores of the chosen, divided by their sum with
+    ``renormalize``, times ``scale``.
+
+    A logit of -inf or NaN (or a bias of -inf) makes an expert unavailable. Where fewer than k
+    are available the remaining ids are -1 with weight 0, which ``dispatch`` skips. +inf counts
+    as the largest finite value. E <= 1024, k <= 32, num_groups <= 32.
+    """
+    if scoring not in ('sigmoid', 'softmax'):
+        raise ValueError(f"unknown scoring {scoring!r}; expected 'sigmoid' or 'softmax'")
+    if group_score not in ('top2', 'max'):
+        raise ValueError(f"unknown group_score {group_score!r}; expected 'top2' or 'max'")
+    if not logits.is_cuda:
+        if available():   # the argument checks
+            load().router_gate(logits, k, scoring == 'sigmoid', bias, num_groups, topk_groups, group_score == 'top2',
+                               renormalize, scale)
+        return router_gate_reference(logits, k, scoring, bias, num_groups, topk_groups, group_score, renormalize, scale)
+    return load().router_gate(logits, k, scoring == 'sigmoid', bias, num_groups, topk_groups, group_score == 'top2',
+                              renormalize, scale)
+
+
+def router_gate_bwd(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, scoring: str = 'sigmoid',
+                    renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient w.r.t. the logits ([T, E], their type) of ``router_gate``'s weights, with ``idx`` its
+    ids and ``dw`` [T, k] the weights' gradient. The selection is a constant and the bias has no
+    gradient. Ids outside [0, E) (the -1 of unfilled slots) count for nothing."""
+    if scoring not in ('sigmoid', 'softmax'):
+        raise ValueError(f"unknown scoring {scoring!r}; expected 'sigmoid' or 'softmax'")
+    if not logits.is_cuda:
+        if available():   # the argument checks
+            load().router_gate_bwd(logits, idx.contiguous(), dw.float().contiguous(), scoring == 'sigmoid', renormalize,
+                                   scale)
+        return router_gate_bwd_reference(logits, idx, dw, scoring, renormalize, scale)
+    return load().router_gate_bwd(logits, idx.contiguous(), dw.float().contiguous(), scoring == 'sigmoid', renormalize,
+                                  scale)
 
 
 def permute(x, local_ids: torch.Tensor, num_local_experts: int, counts: list[int] | None = None,

@@ -122,6 +122,28 @@ def dequantize_fp8_1x128(q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return (qf * s.unsqueeze(-1)).reshape(q.shape)
 
 
+def quantize_fp8_128x128(w: torch.Tensor):
+    """e4m3 with one fp32 scale per 128 x 128 block of ``w`` [.., N, K] (torch definition of the
+    weight quantiser; the last blocks of a side may be short). Constants as in the 1x128 form."""
+    *lead, N, K = w.shape
+    B = FP8_BLOCK
+    wf = torch.nn.functional.pad(w.float(), (0, -K % B, 0, -N % B))
+    wf = wf.reshape(*lead, -(-N // B), B, -(-K // B), B)
+    amax = wf.abs().amax((-3, -1)).clamp_min(FP8_AMAX_FLOOR)
+    c448 = torch.full_like(amax, FP8_MAX)
+    inv = torch.div(c448, amax)
+    q = (wf * inv[..., :, None, :, None]).clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
+    q = q.reshape(*lead, -(-N // B) * B, -(-K // B) * B)[..., :N, :K].contiguous()
+    return q, torch.div(amax, c448)
+
+
+def dequantize_fp8_128x128(q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """fp32 of e4m3 ``q`` [.., N, K] times its 128 x 128 block scales."""
+    N, K = q.shape[-2:]
+    s = scales.repeat_interleave(FP8_BLOCK, -2).repeat_interleave(FP8_BLOCK, -1)
+    return q.float() * s[..., :N, :K]
+
+
 def float_to_ue8m0(scales: torch.Tensor) -> torch.Tensor:
     """Power-of-two fp32 scales -> packed UE8M0 bytes (4 blocks per int32 when H % 512 == 0)."""
     exp = ((scales.contiguous().view(torch.int32) >> 23) & 0xFF).to(torch.uint8)

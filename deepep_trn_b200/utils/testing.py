@@ -77,6 +77,82 @@ def router_topk_reference(logits: torch.Tensor, topk: int):
     return idx.to(torch.int64), w
 
 
+def _check_gate(E: int, k: int, num_groups: int, topk_groups: int):
+    if not (1 <= topk_groups <= num_groups <= 32 and E % num_groups == 0):
+        raise RuntimeError('need 1 <= topk_groups <= num_groups <= 32 and num_groups dividing E')
+    if not 1 <= k <= min(32, E // num_groups * topk_groups):
+        raise RuntimeError('need 1 <= k <= 32 and k <= the experts of the chosen groups')
+
+
+def _gate_scores(logits: torch.Tensor, scoring: str):
+    """Logits in fp64 (NaN -> -inf, +inf -> the largest fp32) and their scores."""
+    x = logits.double()
+    x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x).clamp_max(torch.finfo(torch.float32).max)
+    if scoring == 'sigmoid':
+        return x, torch.sigmoid(x)
+    top = x.amax(1, keepdim=True).clamp_min(-1e300)
+    e = torch.exp(x - top)
+    return x, e / e.sum(1, keepdim=True).clamp_min(1e-300)
+
+
+def router_gate_reference(logits: torch.Tensor, k: int, scoring: str = 'sigmoid', bias=None, num_groups: int = 1,
+                          topk_groups: int = 1, group_score: str = 'top2', renormalize: bool = True,
+                          scale: float = 1.0):
+    """Torch definition of the expert gate (fp64 throughout, weights rounded to fp32 once)."""
+    T, E = logits.shape
+    _check_gate(E, k, num_groups, topk_groups)
+    x, s = _gate_scores(logits, scoring)
+    # both scores grow with the logit: without a bias or a sum, the logits' order is the exact one
+    c = x if bias is None and (num_groups == 1 or group_score == 'max') else s if bias is None else s + bias.double()
+    c = torch.where((x > -math.inf) & ~torch.isnan(c), c, torch.full_like(c, -math.inf))
+    if num_groups > 1:
+        top = torch.sort(c.view(T, num_groups, -1), dim=2, descending=True).values
+        gs = top[..., 0]
+        if group_score == 'top2' and top.shape[2] > 1:
+            gs = torch.where(top[..., 1] > -math.inf, gs + top[..., 1], gs)
+        order = torch.sort(gs, dim=1, descending=True, stable=True).indices[:, :topk_groups]
+        keep = torch.zeros(T, num_groups, dtype=torch.bool, device=c.device).scatter_(1, order, True)
+        c = c.masked_fill(~keep.repeat_interleave(E // num_groups, 1), -math.inf)
+    vals, idx = torch.sort(c, dim=1, descending=True, stable=True)
+    vals, idx = vals[:, :k], idx[:, :k]
+    has = vals > -math.inf
+    w = torch.where(has, s.gather(1, idx), torch.zeros_like(vals))
+    if renormalize:
+        # of sigmoid scores the quotient is formed from logarithms: all may underflow
+        ls = torch.nn.functional.logsigmoid(x) if scoring == 'sigmoid' else x
+        ls = torch.where(has, ls.gather(1, idx), torch.full_like(vals, -math.inf))
+        e = torch.exp(ls - ls.amax(1, keepdim=True).clamp_min(-1e300))
+        w = e / e.sum(1, keepdim=True).clamp_min(1e-300)
+    return torch.where(has, idx, -torch.ones_like(idx)), (w * scale).float()
+
+
+def router_gate_bwd_reference(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, scoring: str = 'sigmoid',
+                              renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Torch definition of the gate's gradient (fp64, rounded to the logits' type once)."""
+    x, s = _gate_scores(logits, scoring)
+    E = x.shape[1]
+    has = (idx >= 0) & (idx < E)
+    at = idx.clamp(0, E - 1)
+    has = has & (x.gather(1, at) > -math.inf)
+    zero = torch.zeros(idx.shape, dtype=torch.float64, device=x.device)
+    g = torch.where(has, dw.double() * scale, zero)
+    if not renormalize and scoring == 'softmax':
+        full = torch.zeros_like(x).scatter_add_(1, at, g)
+        return (s * (full - (full * s).sum(1, keepdim=True))).to(logits.dtype)
+    sk = torch.where(has, s.gather(1, at), zero)
+    if renormalize:
+        ls = torch.nn.functional.logsigmoid(x) if scoring == 'sigmoid' else x
+        ls = torch.where(has, ls.gather(1, at), torch.full_like(zero, -math.inf))
+        e = torch.exp(ls - ls.amax(1, keepdim=True).clamp_min(-1e300))
+        p = e / e.sum(1, keepdim=True).clamp_min(1e-300)
+        g = p * (g - (p * g).sum(1, keepdim=True))
+        if scoring == 'sigmoid':
+            g = g * (1 - sk)
+    else:
+        g = g * sk * (1 - sk)
+    return torch.zeros_like(x).scatter_add_(1, at, torch.where(has, g, zero)).to(logits.dtype)
+
+
 def randn_router(tokens: int, experts: int, topk: int, seed: int, device='cpu'):
     """randn logits [T, E] -> top-k with softmax over the chosen k."""
     gen = torch.Generator().manual_seed(seed)
