@@ -9,8 +9,9 @@
 //     T[i, j] = sum_{k in block} a_ik b_jk ,
 // and the epilogue warps add sa[i, block] * sb[j / 128, block] * T[i, j] to sums that stay in
 // their registers for the whole of K, while the next block is multiplied into the other of two
-// TMEM buffers. Per 128 x 256 tile and block that is 32 KFMA on the CUDA cores, as pairs
-// (fma.rn.f32x2) 128 issue cycles a scheduler against the 512 cycles of the four MMAs.
+// TMEM buffers. Per 128 x 256 tile and block that is 32 KFMA on the CUDA cores, 256 cycles of
+// their pipes against the 512 cycles of the four MMAs (packed fma.rn.f32x2 has the same rate, and
+// cost a move for almost every pair).
 //
 // Rows come as segments (offsets) or as G slabs of `cap` rows of which counts[g] are in use
 // (masked, what a low-latency dispatch delivers); rows outside a group are neither written nor
@@ -20,7 +21,7 @@
 // columns, so it holds whole 128-blocks of h = silu(gate) * up, which leave as e4m3 with one
 // fp32 scale per row and block (scale = max(amax, 1e-4) / 448), the operand of the next product.
 //
-// 12 warps: TMA producer, TMEM owner + MMA issuer, two idle, 8 epilogue warps (two per TMEM lane quarter,
+// 12 warps: TMA producer, two MMA issuers (warp 1 owns the TMEM), a scale warp, 8 epilogue warps (two per TMEM lane quarter,
 // 128 columns each). Every wait is bounded; a wait that runs out sets *error, lets the copies in
 // flight land, frees the TMEM and returns.
 #include <ATen/cuda/CUDAContext.h>
@@ -37,12 +38,12 @@ constexpr int kBM = 128, kBN = 256, kBK = 128;   // tile; kBK one-byte elements 
 constexpr int kStages = 4;
 constexpr int kABytes = kBM * kBK, kBBytes = kBN * kBK, kStageBytes = kABytes + kBBytes;
 constexpr int kEpiWarps = 8;
-constexpr int kFirstEpi = 4;                     // warps 0 and 1 load and multiply, 2 and 3 only lend registers
+constexpr int kFirstEpi = 4;                     // warps 0 to 3: loads, MMAs, scales
 constexpr int kBlkThreads = 32 * (kFirstEpi + kEpiWarps);
 // Registers a thread: 128 sums and their operands need more than an even split of the file
 // (168). The first warpgroup gives up what the two epilogue warpgroups take:
-// 128 * 64 + 256 * 208 = 61440 of the 384 * 168 = 64512 the block is launched with.
-constexpr int kRegsMain = 64, kRegsEpi = 208;
+// 128 * 72 + 256 * 216 = 64512 = 384 * 168, what the block is launched with.
+constexpr int kRegsMain = 72, kRegsEpi = 216;
 constexpr int kWarpStage = 32 * 64;              // a warp's output staging: 64 bytes of its 32 rows
 constexpr int kMaxG = 1024;
 
@@ -79,48 +80,57 @@ __device__ __forceinline__ void tc_mma_fp8(uint32_t tmem_d, uint64_t adesc, uint
 __host__ __device__ constexpr uint32_t idesc_fp8(int n, bool b_mn) {
   return (1u << 4) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
 }
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-  return d;
+// One lane of a converged warp, in the form from which the compiler knows that a single thread issues
+// what follows (behind `lane == 0` it guards every tcgen05 and TMA instruction against a diverged warp).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
 }
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-  uint32_t a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-  lo = __uint_as_float(a);
-  hi = __uint_as_float(b);
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void* smem, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(src), "n"(BYTES) : "memory");
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
+// Bounded wait (the clock and the abort flag are looked at once in 256 polls). Every hand-over between
+// warps through an mbarrier takes about 130 cycles; with a suspend-time hint it took longer still.
 __device__ __forceinline__ bool wait_blk(uint64_t* bar, uint32_t parity, const BlkArgs& a, volatile int* abort) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*abort || global_ns() - t0 > a.timeout_ns) {
-      atomicExch(a.error, 1u);
-      *abort = 1;
-      return false;
+  uint64_t t0 = 0;
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 255u) == 0u) {
+      const uint64_t now = global_ns();
+      if (t0 == 0) t0 = now;
+      if (*abort || now - t0 > a.timeout_ns) {
+        atomicExch(a.error, 1u);
+        *abort = 1;
+        return false;
+      }
     }
   }
-  return true;
 }
 
 struct Groups {
-  int base[kMaxG];       // first row (segments) or 0
   int cnt[kMaxG];        // rows in use
   int pref[kMaxG + 1];   // m tiles of the groups before
 };
 
+// First row of a group (0 for slabs), clamped to the buffer.
+__device__ __forceinline__ int64_t group_base(const BlkArgs& a, int g) {
+  if (a.offsets == nullptr) return 0;
+  const int64_t lo = a.offsets[g], top = a.rows;
+  return lo < 0 ? 0 : (lo > top ? top : lo);
+}
+
 // Rows and m tiles of every group, from the device's offsets / counts, clamped to the buffer.
 __device__ __forceinline__ void load_groups(Groups& s, const BlkArgs& a) {
   for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-    int64_t b = 0, c = a.rows;
+    int64_t c = a.rows;
     if (a.offsets != nullptr) {
-      const int64_t lo = a.offsets[g], hi = a.offsets[g + 1], top = a.rows;
-      b = lo < 0 ? 0 : (lo > top ? top : lo);
+      const int64_t hi = a.offsets[g + 1], top = a.rows, b = group_base(a, g);
       const int64_t e = hi > top ? top : hi;
       c = e > b ? e - b : 0;
     }
@@ -128,7 +138,6 @@ __device__ __forceinline__ void load_groups(Groups& s, const BlkArgs& a) {
       const int64_t n = a.counts[g];
       c = n < 0 ? 0 : (n < c ? n : c);
     }
-    s.base[g] = static_cast<int>(b);
     s.cnt[g] = static_cast<int>(c);
   }
   __syncthreads();
@@ -176,7 +185,9 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
   uint8_t* sB = sA + kStages * kABytes;
   uint8_t* sE = sB + kStages * kBBytes;
   __shared__ Groups s_grp;
-  __shared__ uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], drain;
+  __shared__ uint64_t full[kStages], empty[kStages], tfull[2], tempty[2], drain[2];
+  __shared__ __align__(16) float s_sa[2][kBM][4], s_sb[2][2][4];   // scales as they come, four K blocks a unit
+  __shared__ float s_scale[2][2][kBM];   // sa * sb of the block in a TMEM buffer: [buffer][128-column half][row]
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int s_abort;
   __shared__ uint32_t s_amax[2][2][kBM];   // [tile parity][column half][row]
@@ -189,10 +200,10 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&tfull[b], 1);
+      mbar_init(&tfull[b], 2);   // the MMAs' commit and the scale warp
       mbar_init(&tempty[b], kEpiWarps);
+      mbar_init(&drain[b], 1);
     }
-    mbar_init(&drain, 1);
     fence_mbar_init();
     prefetch_tmap(&tmA);
     prefetch_tmap(&tmB);
@@ -209,15 +220,15 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsMain));
     if (warp == 0) {
       // ------------------------------------------------------------------ TMA producer
-      if (lane == 0) {
-        uint32_t it = 0;
-        BlkTile tl;
-        for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
-          const int row = a.offsets != nullptr ? s_grp.base[tl.g] + tl.m0 : tl.m0;
-          const int slab = a.offsets != nullptr ? 0 : tl.g;
-          for (int kb = 0; kb < KB; ++kb, ++it) {
-            const int s = it % kStages;
-            if (!wait_blk(&empty[s], ((it / kStages) & 1u) ^ 1u, a, &s_abort)) break;
+      uint32_t it = 0;
+      BlkTile tl;
+      for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
+        const int row = static_cast<int>(group_base(a, tl.g)) + tl.m0;
+        const int slab = a.offsets != nullptr ? 0 : tl.g;
+        for (int kb = 0; kb < KB; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!wait_blk(&empty[s], ((it / kStages) & 1u) ^ 1u, a, &s_abort)) break;
+          if (elect_one()) {
             mbar_arrive_expect_tx(&full[s], kStageBytes);
             tma_load_3d(sA + s * kABytes, &tmA, &full[s], kb * kBK, row, slab);
             uint8_t* db = sB + s * kBBytes;
@@ -229,38 +240,116 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
               tma_load_3d(db, &tmB, &full[s], kb * kBK, tl.n0, tl.g);
             }
           }
-        }
-        if (s_abort) {  // copies in flight land before the CTA's shared memory is given up
-          for (uint32_t q = it > kStages ? it - kStages : 0; q < it; ++q)
-            mbar_wait(&full[q % kStages], (q / kStages) & 1u, 1000000000ull);
+          __syncwarp();
         }
       }
-    } else if (warp == 1) {
-      // ------------------------------------------------------------------ MMA issuer
-      if (lane == 0) {
-        constexpr uint32_t idesc = idesc_fp8(kBN, B_MN);
-        uint32_t it = 0;
-        BlkTile tl;
-        for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
-          for (int kb = 0; kb < KB; ++kb, ++it) {
-            const int s = it % kStages, b = it & 1;
-            if (!wait_blk(&tempty[b], ((it >> 1) & 1u) ^ 1u, a, &s_abort)) break;
-            if (!wait_blk(&full[s], (it / kStages) & 1u, a, &s_abort)) break;
-            tc_fence_after();
-            const uint64_t ad = smem_desc_k128(sA + s * kABytes);
-            const uint64_t bd = B_MN ? smem_desc_mn128(sB + s * kBBytes, 128 * kBK) : smem_desc_k128(sB + s * kBBytes);
+      if (s_abort) {  // copies in flight land before the CTA's shared memory is given up
+        for (uint32_t q = it > kStages ? it - kStages : 0; q < it; ++q)
+          mbar_wait(&full[q % kStages], (q / kStages) & 1u, 1000000000ull);
+      }
+    } else if (warp <= 2) {
+      // ------------------------------------------------------------------ MMA issuers
+      // one warp for each TMEM buffer: the waits and the issue of a K block's MMAs take one warp
+      // longer than the MMAs themselves
+      const uint32_t b = warp - 1;
+      constexpr uint32_t idesc = idesc_fp8(kBN, B_MN);
+      uint32_t it = 0;
+      BlkTile tl;
+      for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
+        for (int kb = 0; kb < KB; ++kb, ++it) {
+          if ((it & 1u) != b) continue;
+          const int s = it % kStages;
+          // the buffer comes last: from its release on every cycle delays the next block
+          if (!wait_blk(&full[s], (it / kStages) & 1u, a, &s_abort)) break;
+          const uint64_t ad = smem_desc_k128(sA + s * kABytes);
+          const uint64_t bd = B_MN ? smem_desc_mn128(sB + s * kBBytes, 128 * kBK) : smem_desc_k128(sB + s * kBBytes);
+          if (!wait_blk(&tempty[b], ((it >> 1) & 1u) ^ 1u, a, &s_abort)) break;
+          tc_fence_after();
+          if (elect_one()) {
             // next 32 channels: 32 bytes along a K-major swizzle row, or 32 rows of 128 bytes
             constexpr uint64_t bstep = B_MN ? (32 * 128) >> 4 : 2;
 #pragma unroll
             for (int k = 0; k < kBK / 32; ++k)
               tc_mma_fp8(tmem_base + b * kBN, ad + 2 * k, bd + bstep * k, idesc, k > 0 ? 1u : 0u);
-            tc_commit(&empty[s]);
             tc_commit(&tfull[b]);
+            tc_commit(&empty[s]);
+          }
+          __syncwarp();
+        }
+      }
+      if (elect_one()) tc_commit(&drain[b]);  // every MMA issued is done before TMEM is released
+      __syncwarp();
+      mbar_wait(&drain[b], 0, a.timeout_ns);
+    } else {
+      // ------------------------------------------------------------------ scales (warp 3)
+      // The scales of four K blocks (of the tile's 128 rows and two column blocks) are copied
+      // asynchronously, a unit ahead of their use and across tiles, 16 bytes a row where the rows
+      // of sa allow it; their products go to the epilogue with the block's TMEM buffer.
+      const int NB = (a.N + 127) / 128;
+      const bool wide = ((reinterpret_cast<uintptr_t>(a.sa) | (a.sa_row * 4) | (a.sa_group * 4)) & 15) == 0;
+      int t = blockIdx.x, k0 = 0;      // the unit to be copied next
+      BlkTile tl;
+      bool left = blk_tile(t, a, s_grp, tl);
+      auto copy_unit = [&](int s) {
+        if (left) {
+          const int cnt = s_grp.cnt[tl.g];
+          const float* sa = a.sa + tl.g * a.sa_group + group_base(a, tl.g) * a.sa_row;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* src = sa + min(tl.m0 + 32 * i + lane, cnt - 1) * a.sa_row + k0;
+            float* dst = s_sa[s][32 * i + lane];
+            if (wide && k0 + 4 <= KB) {
+              cp_async<16>(dst, src);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (k0 + j < KB) cp_async<4>(dst + j, src + j);
+            }
+          }
+          // lane h * 4 + j < 8 copies block j of column block h
+          const float* sb = a.sb + tl.g * a.sb_group + min(tl.n0 / 128 + (lane >> 2 & 1), NB - 1) * a.sb_n;
+          if (lane < 8 && k0 + (lane & 3) < KB)
+            cp_async<4>(&s_sb[s][lane >> 2][lane & 3], sb + (k0 + (lane & 3)) * a.sb_k);
+          k0 += 4;
+          if (k0 >= KB) {
+            k0 = 0;
+            t += gridDim.x;
+            left = blk_tile(t, a, s_grp, tl);
           }
         }
-        tc_commit(&drain);  // every MMA issued is done before TMEM is released
-        mbar_wait(&drain, 0, a.timeout_ns);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      copy_unit(0);
+      copy_unit(1);
+      uint32_t it = 0, u = 0;
+      bool ok = true;
+      BlkTile at;
+      for (int tt = blockIdx.x; ok && !s_abort && blk_tile(tt, a, s_grp, at); tt += gridDim.x) {
+        for (int kb = 0; kb < KB && ok; ++kb, ++it) {
+          const int s = u & 1, j = kb & 3, b = it & 1;
+          if (j == 0) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();
+          }
+          float f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = s_sa[s][32 * i + lane][j];
+          const float b0 = s_sb[s][0][j], b1 = s_sb[s][1][j];
+          ok = wait_blk(&tempty[b], ((it >> 1) & 1u) ^ 1u, a, &s_abort);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s_scale[b][0][32 * i + lane] = f[i] * b0;
+            s_scale[b][1][32 * i + lane] = f[i] * b1;
+          }
+          __syncwarp();
+          if (lane == 0 && ok) mbar_arrive(&tfull[b]);
+          if (j == 3 || kb + 1 == KB) {
+            copy_unit(s);
+            ++u;
+          }
+        }
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
@@ -272,57 +361,59 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
     auto col_of = [half](int c) {
       return EPI == kOutSwiGLU ? (c < 2 ? half * 64 + 32 * c : 128 + half * 64 + 32 * (c - 2)) : half * 128 + 32 * c;
     };
-    const int NB = (a.N + 127) / 128;
+    const uint32_t tq = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
     uint32_t it = 0;
     int parity = 0;
     BlkTile tl;
     for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x, parity ^= 1) {
       const int cnt = s_grp.cnt[tl.g];
       const int row = tl.m0 + q * 32 + lane;           // within the group
-      const int64_t arow = s_grp.base[tl.g] + min(row, cnt - 1);
-      const float* sa = a.sa + tl.g * a.sa_group + arow * a.sa_row;
-      const int nb = tl.n0 / 128;
-      const int nb0 = EPI == kOutSwiGLU ? nb : min(nb + half, NB - 1);
-      const int nb1 = EPI == kOutSwiGLU ? nb + 1 : nb0;
-      const float* sb0 = a.sb + tl.g * a.sb_group + nb0 * a.sb_n;
-      const float* sb1 = a.sb + tl.g * a.sb_group + nb1 * a.sb_n;
-      uint64_t acc[64];
+      const int64_t base = group_base(a, tl.g);
+      float acc[128];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = 0;
-      float na = sa[0], n0s = sb0[0], n1s = sb1[0];
-      bool ok = true;
-      for (int kb = 0; kb < KB; ++kb, ++it) {
-        const int b = it & 1;
-        const float f0 = na * n0s, f1 = EPI == kOutSwiGLU ? na * n1s : f0;
-        if (kb + 1 < KB) {
-          na = sa[kb + 1];
-          n0s = sb0[(kb + 1) * a.sb_k];
-          if (EPI == kOutSwiGLU) n1s = sb1[(kb + 1) * a.sb_k];
-        }
-        if (!wait_blk(&tfull[b], (it >> 1) & 1u, a, &s_abort)) {
-          ok = false;
-          break;
-        }
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      // A block's four 32-column chunks go through two register buffers, two loads in flight; the
+      // TMEM buffer is handed back once the last is in, with half of the sums still to be added, and
+      // the next block's first loads leave before the last chunk is added.
+      uint32_t r[2][32];
+      bool ok;
+      auto add = [&](int c, float f) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(r[c & 1][i]), f, acc[c * 32 + i]);
+      };
+      float f0 = 0.f, f1 = 0.f;
+      auto begin_block = [&]() {   // block `it`: its first chunk and its scales
+        ok = wait_blk(&tfull[it & 1], (it >> 1) & 1u, a, &s_abort);
         tc_fence_after();
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * kBN;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t r[32];
-          tmem_ld32(taddr + col_of(c), r);
-          const uint32_t f = __float_as_uint(c < 2 ? f0 : f1);
-          const uint64_t ff = pack2(f, f);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) acc[c * 16 + i] = fma2(pack2(r[2 * i], r[2 * i + 1]), ff, acc[c * 16 + i]);
-        }
+        if (ok) tmem_ld32_async(tq + (it & 1) * kBN + col_of(0), r[0]);
+        f0 = s_scale[it & 1][EPI == kOutSwiGLU ? 0 : half][q * 32 + lane];
+        f1 = EPI == kOutSwiGLU ? s_scale[it & 1][1][q * 32 + lane] : f0;
+      };
+      begin_block();
+#pragma unroll 1
+      for (int kb = 0; kb < KB && ok; ++kb) {
+        const uint32_t taddr = tq + (it & 1) * kBN;
+        tmem_ld32_async(taddr + col_of(1), r[1]);
+        tmem_wait_ld64(r[0], r[1]);
+        add(0, f0);
+        tmem_ld32_async(taddr + col_of(2), r[0]);
+        add(1, f0);
+        tmem_ld32_async(taddr + col_of(3), r[1]);
+        tmem_wait_ld64(r[0], r[1]);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&tempty[b]);
+        if (lane == 0) mbar_arrive(&tempty[it & 1]);
+        ++it;
+        const float f = f1;
+        add(2, f);
+        if (kb + 1 < KB) begin_block();
+        add(3, f);
       }
       if (!ok) break;
       // ---- output: 64 bytes of each of the warp's 32 rows at a time, through shared memory (the
       // 16-byte pieces of a row are swapped by row pair, so that 8 lanes hit distinct banks)
       const int first = tl.m0 + q * 32;
-      const int64_t grow = s_grp.base[tl.g] + first;
+      const int64_t grow = base + first;
       auto store64 = [&](uint8_t* base, int64_t row_stride, int ncols16, const uint32_t (&v)[16]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -344,12 +435,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
           const int col = tl.n0 + half * 128 + 16 * c;
           uint32_t v[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float x, y;
-            unpack2(acc[c * 8 + i], x, y);
-            v[2 * i] = __float_as_uint(x);
-            v[2 * i + 1] = __float_as_uint(y);
-          }
+          for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(acc[c * 16 + i]);
           store64(crow + 4 * static_cast<int64_t>(col), a.c_row, (a.N - col) / 4, v);
         }
       } else if (EPI == kOutBF16 || a.C != nullptr) {
@@ -358,11 +444,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
           const int col = tl.n0 + col_of(c);
           uint32_t v[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float x, y;
-            unpack2(acc[c * 16 + i], x, y);
-            v[i] = pack_bf16(x, y);
-          }
+          for (int i = 0; i < 16; ++i) v[i] = pack_bf16(acc[c * 32 + 2 * i], acc[c * 32 + 2 * i + 1]);
           store64(crow + 2 * static_cast<int64_t>(col), a.c_row, (a.N - col) / 8, v);
         }
       }
@@ -371,13 +453,9 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
         float h[64];
         uint32_t top = 0;   // as bits, so that a NaN stays the largest
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float g0, g1, u0, u1;
-          unpack2(acc[i], g0, g1);
-          unpack2(acc[32 + i], u0, u1);
-          h[2 * i] = __fdividef(g0, 1.f + __expf(-g0)) * u0;
-          h[2 * i + 1] = __fdividef(g1, 1.f + __expf(-g1)) * u1;
-          top = max(top, max(__float_as_uint(fabsf(h[2 * i])), __float_as_uint(fabsf(h[2 * i + 1]))));
+        for (int i = 0; i < 64; ++i) {
+          h[i] = __fdividef(acc[i], 1.f + __expf(-acc[i])) * acc[64 + i];
+          top = max(top, __float_as_uint(fabsf(h[i])));
         }
         s_amax[parity][half][q * 32 + lane] = top;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");  // this warp and the other half's
