@@ -21,11 +21,22 @@
 // columns, so it holds whole 128-blocks of h = silu(gate) * up, which leave as e4m3 with one
 // fp32 scale per row and block (scale = max(amax, 1e-4) / 448), the operand of the next product.
 //
-// 12 warps: TMA producer, two MMA issuers (warp 1 owns the TMEM), a scale warp, 8 epilogue warps (two per TMEM lane quarter,
-// 128 columns each). Every wait is bounded; a wait that runs out sets *error, lets the copies in
-// flight land, frees the TMEM and returns.
+// Two kernels, for groups with many and with few rows:
+//  * many: 128 rows x 256 columns, rows of A on the TMEM lanes; a CTA takes whole tiles. Bound by the
+//    operands' way into shared memory (48 KB a block at 64 bytes a cycle: 768 cycles).
+//  * few (at most kFewTile rows): 256 columns x up to 48 rows, columns of C on the lanes, so that
+//    nothing is spent on rows that are not there. Bound by reading B. Tiles that do not fill a round of the SMs are taken by clusters that divide
+//    K and add their parts through distributed shared memory in a fixed order.
+// Segments take one of the two, by the rows that there are. For slabs, whose counts only the device
+// knows, both are launched where the second is worth it, and each takes its groups.
+//
+// 12 warps: TMA producer, MMA issuer (one for each TMEM buffer in the kernel for many rows; warp 1 owns
+// the TMEM), a scale warp, 8 epilogue warps. Every wait is bounded; a wait that runs out sets *error,
+// lets the copies in flight land, frees the TMEM and returns.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+
+#include <climits>
 
 #include "ops.h"
 #include "tcgen05.cuh"
@@ -47,7 +58,32 @@ constexpr int kRegsMain = 72, kRegsEpi = 216;
 constexpr int kWarpStage = 32 * 64;              // a warp's output staging: 64 bytes of its 32 rows
 constexpr int kMaxG = 1024;
 
+constexpr int kFewTile = 48;                     // rows of a tile with few rows, and of a group that counts as one
+constexpr int kFewStages = 4, kFewBufs = 4;
+constexpr int kFewCols = 64;                     // TMEM columns of a buffer's half
+constexpr int kFewStageBytes = kBBytes + kFewTile * kBK;
+constexpr int kFewPair = 2;                      // K blocks that are loaded together
+constexpr int kMaxSplit = 8;                     // CTAs of a cluster that divide K
+static_assert(kStages % 2 == 0, "two MMA warps take turns: each must see every phase of its stages' barriers");
+static_assert(kFewTile <= kFewCols && kFewBufs * 2 * kFewCols <= 2 * kBN, "TMEM columns");
+
+enum Form : int { kBothForms = 0, kAllMany = 1, kAllFew = 2 };
 enum BlkEpilogue : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiGLU = 2 };
+
+// Estimated cycles, from measurements. A K block of a tile takes 900, or 1540 where all SMs read a part of
+// B of their own from memory. A tile with few rows costs 2300 more, and 16000 where a cluster divides K.
+// (Decoding, 32 groups of 32 rows: N 4096, K 7168, 512 tiles: 181 us as many rows, in 4 rounds, 165 as
+// few; N 7168, K 2048, 896 tiles: 91 and 100 us. One row, N 2048, K 7168: 14 and 10.7 us.)
+__host__ __device__ inline int64_t block_cycles(int64_t ctas, int64_t sms, bool own) { return own && ctas * 2 > sms ? 1540 : 900; }
+__host__ __device__ inline int64_t many_cycles(int64_t tiles, int64_t KB, int64_t sms, bool own) {
+  return (tiles + sms - 1) / sms * KB * block_cycles(tiles, sms, own) + 4000;
+}
+__host__ __device__ inline int64_t few_cycles(int64_t tiles, int64_t KB, int64_t grid, int64_t split) {
+  if (split == 1) return (tiles + grid - 1) / grid * (KB * block_cycles(tiles, grid, true) + 2300) + 4000;
+  const int64_t left = tiles % grid, rounds = (left * split + grid - 1) / grid;
+  return tiles / grid * (KB * 1540 + 2300) +
+         rounds * ((KB + split - 1) / split * block_cycles(left * split, grid, true) + 16000) + 4000;
+}
 
 struct BlkArgs {
   const int64_t* offsets;   // [G + 1] or nullptr (masked)
@@ -65,6 +101,8 @@ struct BlkArgs {
   int64_t hs_row, hs_group;
   uint32_t* error;
   uint64_t timeout_ns;
+  int form;                 // Form
+  int sms, split, few_grid; // launch shapes, from which both kernels conclude the same
 };
 
 __device__ __forceinline__ void tc_mma_fp8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -76,9 +114,10 @@ __device__ __forceinline__ void tc_mma_fp8(uint32_t tmem_d, uint64_t adesc, uint
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D fp32, A and B e4m3, M = 128; bit 16 selects an MN-major B
-__host__ __device__ constexpr uint32_t idesc_fp8(int n, bool b_mn) {
-  return (1u << 4) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
+// D fp32, A and B e4m3, M = 128; bits 15 and 16 select an MN-major A and B
+__host__ __device__ constexpr uint32_t idesc_fp8(int n, bool a_mn, bool b_mn) {
+  return (1u << 4) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(n >> 3) << 17) |
+         (uint32_t(kBM >> 4) << 24);
 }
 // One lane of a converged warp, in the form from which the compiler knows that a single thread issues
 // what follows (behind `lane == 0` it guards every tcgen05 and TMA instruction against a diverged warp).
@@ -114,45 +153,71 @@ __device__ __forceinline__ bool wait_blk(uint64_t* bar, uint32_t parity, const B
 }
 
 struct Groups {
-  int cnt[kMaxG];        // rows in use
-  int pref[kMaxG + 1];   // m tiles of the groups before
+  int pref[kMaxG + 1];   // tiles (of rows) of the groups before; none for a group of the other form
+};
+struct Span {
+  int64_t base;          // first row (0 for slabs)
+  int cnt;               // rows in use
 };
 
-// First row of a group (0 for slabs), clamped to the buffer.
-__device__ __forceinline__ int64_t group_base(const BlkArgs& a, int g) {
-  if (a.offsets == nullptr) return 0;
-  const int64_t lo = a.offsets[g], top = a.rows;
-  return lo < 0 ? 0 : (lo > top ? top : lo);
+// A group's rows, from the device's offsets / counts, clamped to the buffer.
+__device__ __forceinline__ Span group_span(const BlkArgs& a, int g) {
+  int64_t b = 0, c = a.rows;
+  if (a.offsets != nullptr) {
+    const int64_t lo = a.offsets[g], hi = a.offsets[g + 1], top = a.rows;
+    b = lo < 0 ? 0 : (lo > top ? top : lo);
+    c = (hi > top ? top : hi) - b;
+    c = c < 0 ? 0 : c;
+  }
+  if (a.counts != nullptr) {
+    const int64_t n = a.counts[g];
+    c = n < 0 ? 0 : (n < c ? n : c);
+  }
+  return {b, static_cast<int>(c)};
 }
 
-// Rows and m tiles of every group, from the device's offsets / counts, clamped to the buffer.
+// The tiles of the groups that this form takes. All CTAs of both kernels come to the same answer.
+template <bool FEW>
 __device__ __forceinline__ void load_groups(Groups& s, const BlkArgs& a) {
-  for (int g = threadIdx.x; g < a.G; g += blockDim.x) {
-    int64_t c = a.rows;
-    if (a.offsets != nullptr) {
-      const int64_t hi = a.offsets[g + 1], top = a.rows, b = group_base(a, g);
-      const int64_t e = hi > top ? top : hi;
-      c = e > b ? e - b : 0;
-    }
-    if (a.counts != nullptr) {
-      const int64_t n = a.counts[g];
-      c = n < 0 ? 0 : (n < c ? n : c);
-    }
-    s.cnt[g] = static_cast<int>(c);
-  }
+  for (int g = threadIdx.x; g < a.G; g += blockDim.x) s.pref[g + 1] = group_span(a, g).cnt;
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int carry = 0;
+    int few_rows = a.form == kAllFew ? INT_MAX : 0;   // most rows of a group that counts as one with few
+    if (a.form == kBothForms) {
+      // all groups as many, all as few, or each by its rows: the least estimate
+      int many = 0, few = 0, many_part = 0, few_part = 0, busy = 0;
+      for (int g = lane; g < a.G; g += 32) {
+        const int n = s.pref[g + 1], m = (n + kBM - 1) / kBM, f = (n + kFewTile - 1) / kFewTile;
+        many += m;
+        few += f;
+        (f > 1 ? many_part : few_part) += f > 1 ? m : f;
+        busy += n > 0;
+      }
+      many = __reduce_add_sync(0xffffffffu, many);
+      few = __reduce_add_sync(0xffffffffu, few);
+      many_part = __reduce_add_sync(0xffffffffu, many_part);
+      few_part = __reduce_add_sync(0xffffffffu, few_part);
+      busy = __reduce_add_sync(0xffffffffu, busy);
+      const int64_t ntn = (a.N + kBN - 1) / kBN, KB = (a.K + kBK - 1) / kBK;
+      const int64_t as_many = many_cycles(many * ntn, KB, a.sms, many == busy);
+      const int64_t as_few = few_cycles(few * ntn, KB, a.few_grid, a.split);
+      const int64_t mixed = few_cycles(few_part * ntn, KB, a.few_grid, a.split) +
+                            many_cycles(many_part * ntn, KB, a.sms, many_part == busy - few_part);
+      few_rows = as_few <= min(as_many, mixed) ? INT_MAX : mixed < as_many ? kFewTile : 0;
+    }
+    int total = 0;
     for (int g0 = 0; g0 < a.G; g0 += 32) {
-      int v = g0 + lane < a.G ? (s.cnt[g0 + lane] + kBM - 1) / kBM : 0;
+      const int g = g0 + lane, n = g < a.G ? s.pref[g + 1] : 0;
+      const bool is_few = n <= few_rows;
+      int v = is_few != FEW ? 0 : FEW ? (n + kFewTile - 1) / kFewTile : (n + kBM - 1) / kBM;
 #pragma unroll
       for (int m = 1; m < 32; m <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, v, m);
         if (lane >= m) v += o;
       }
-      if (g0 + lane < a.G) s.pref[g0 + lane + 1] = carry + v;
-      carry += __shfl_sync(0xffffffffu, v, 31);
+      if (g < a.G) s.pref[g + 1] = total + v;
+      total += __shfl_sync(0xffffffffu, v, 31);
     }
     if (lane == 0) s.pref[0] = 0;
   }
@@ -161,21 +226,124 @@ __device__ __forceinline__ void load_groups(Groups& s, const BlkArgs& a) {
 struct BlkTile {
   int g, m0, n0;
 };
+// The last group whose share begins at or before t, where a tile of rows counts `per` times.
+__device__ __forceinline__ int group_of(int t, int per, const BlkArgs& a, const Groups& s) {
+  int lo = 0, hi = a.G - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s.pref[mid] * per <= t) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
 __device__ __forceinline__ bool blk_tile(int t, const BlkArgs& a, const Groups& s, BlkTile& tl) {
   const int ntn = (a.N + kBN - 1) / kBN;
   const int mt = t / ntn;
   if (mt >= s.pref[a.G]) return false;
-  int lo = 0, hi = a.G - 1;   // last group with pref[g] <= mt
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (s.pref[mid] <= mt) lo = mid; else hi = mid - 1;
-  }
-  tl.g = lo;
-  tl.m0 = (mt - s.pref[lo]) * kBM;
+  tl.g = group_of(mt, 1, a, s);
+  tl.m0 = (mt - s.pref[tl.g]) * kBM;
   tl.n0 = (t - mt * ntn) * kBN;
   return true;
 }
+// The work of one CTA on groups with few rows: whole tiles for as many rounds as all CTAs have one,
+// then its share of the K blocks of the tiles left over, a cluster to a tile. The row tiles of one
+// column tile follow one another, so that B is read once from memory. The next tile is looked up
+// while the current one is worked on.
+struct FewTiles {
+  const BlkArgs& a;
+  const Groups& s;
+  int whole, tiles;      // tiles [0, whole) go to single CTAs, [whole, tiles) to clusters
+  int crank, csize, KB;
+  int t;                 // the next tile's number
+  BlkTile tl, next;
+  Span sp, next_sp;
+  int k0, k1, next_k0, next_k1;   // its K blocks
+  bool split, next_split, more;
+  __device__ __forceinline__ FewTiles(const BlkArgs& a, const Groups& s, int crank, int csize)
+      : a(a), s(s), crank(crank), csize(csize), KB((a.K + kBK - 1) / kBK) {
+    tiles = s.pref[a.G] * ((a.N + kBN - 1) / kBN);
+    whole = csize > 1 ? tiles / static_cast<int>(gridDim.x) * static_cast<int>(gridDim.x) : tiles;
+    t = blockIdx.x;
+    if (t >= whole) t = whole + blockIdx.x / csize;
+    find();
+  }
+  __device__ __forceinline__ void find() {
+    more = t < tiles;
+    if (!more) return;
+    const int ntn = (a.N + kBN - 1) / kBN;
+    const int g = group_of(t, ntn, a, s);
+    next_sp = group_span(a, g);
+    const int rows = s.pref[g + 1] - s.pref[g], r = t - s.pref[g] * ntn;
+    const int col = rows == 1 ? r : r / rows;
+    next.g = g;
+    next.n0 = col * kBN;
+    next.m0 = (r - col * rows) * kFewTile;
+    next_split = t >= whole && csize > 1;
+    next_k0 = next_split ? static_cast<int>(static_cast<int64_t>(KB) * crank / csize) : 0;
+    next_k1 = next_split ? static_cast<int>(static_cast<int64_t>(KB) * (crank + 1) / csize) : KB;
+    if (next_split) {
+      t += gridDim.x / csize;
+    } else {
+      t += gridDim.x;
+      if (t >= whole && csize > 1) t = whole + blockIdx.x / csize;
+    }
+  }
+  __device__ __forceinline__ bool advance() {
+    if (!more) return false;
+    tl = next;
+    sp = next_sp;
+    k0 = next_k0;
+    k1 = next_k1;
+    split = next_split;
+    find();
+    return true;
+  }
+};
+// Address of this CTA's shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_peer(const void* bar, uint32_t rank) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_addr(bar, rank)) : "memory");
+}
+__device__ __forceinline__ float4 load_peer(const float* p, uint32_t rank) {
+  float4 v;
+  // volatile: kept behind the wait and the fence before it
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(peer_addr(p, rank)));
+  return v;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Barrier of `n` threads that tells each whether all of them are well: warps that share a barrier leave
+// together or not at all, so that none is left waiting after a timeout.
+__device__ __forceinline__ bool bar_all(int id, int n, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(ok)), "r"(id), "r"(n)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + __expf(-g)) * u; }
+// The scales of four K blocks (k0 .. k0 + 3 < k1) of one row of sa.
+__device__ __forceinline__ void copy_scales(float* dst, const float* src, int k0, int k1, bool wide) {
+  if (wide && k0 + 4 <= k1 && (k0 & 3) == 0) {
+    cp_async<16>(dst, src);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (k0 + j < k1) cp_async<4>(dst + j, src + j);
+  }
+}
 
+// ------------------------------------------------------------------------------ groups with many rows
 template <int EPI, bool B_MN>
 __global__ void __launch_bounds__(kBlkThreads, 1)
     gemm_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, BlkArgs a) {
@@ -209,7 +377,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
     prefetch_tmap(&tmB);
   }
   if (warp == 1) tmem_alloc(&tmem_slot, 2 * kBN);
-  load_groups(s_grp, a);
+  load_groups<false>(s_grp, a);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -223,7 +391,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       uint32_t it = 0;
       BlkTile tl;
       for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
-        const int row = static_cast<int>(group_base(a, tl.g)) + tl.m0;
+        const int row = static_cast<int>(group_span(a, tl.g).base) + tl.m0;
         const int slab = a.offsets != nullptr ? 0 : tl.g;
         for (int kb = 0; kb < KB; ++kb, ++it) {
           const int s = it % kStages;
@@ -252,7 +420,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       // one warp for each TMEM buffer: the waits and the issue of a K block's MMAs take one warp
       // longer than the MMAs themselves
       const uint32_t b = warp - 1;
-      constexpr uint32_t idesc = idesc_fp8(kBN, B_MN);
+      constexpr uint32_t idesc = idesc_fp8(kBN, false, B_MN);
       uint32_t it = 0;
       BlkTile tl;
       for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
@@ -290,22 +458,13 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       int t = blockIdx.x, k0 = 0;      // the unit to be copied next
       BlkTile tl;
       bool left = blk_tile(t, a, s_grp, tl);
+      Span sp = left ? group_span(a, tl.g) : Span{0, 0};
       auto copy_unit = [&](int s) {
         if (left) {
-          const int cnt = s_grp.cnt[tl.g];
-          const float* sa = a.sa + tl.g * a.sa_group + group_base(a, tl.g) * a.sa_row;
+          const float* sa = a.sa + tl.g * a.sa_group + sp.base * a.sa_row + k0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float* src = sa + min(tl.m0 + 32 * i + lane, cnt - 1) * a.sa_row + k0;
-            float* dst = s_sa[s][32 * i + lane];
-            if (wide && k0 + 4 <= KB) {
-              cp_async<16>(dst, src);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (k0 + j < KB) cp_async<4>(dst + j, src + j);
-            }
-          }
+          for (int i = 0; i < 4; ++i)
+            copy_scales(s_sa[s][32 * i + lane], sa + min(tl.m0 + 32 * i + lane, sp.cnt - 1) * a.sa_row, k0, KB, wide);
           // lane h * 4 + j < 8 copies block j of column block h
           const float* sb = a.sb + tl.g * a.sb_group + min(tl.n0 / 128 + (lane >> 2 & 1), NB - 1) * a.sb_n;
           if (lane < 8 && k0 + (lane & 3) < KB)
@@ -315,6 +474,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
             k0 = 0;
             t += gridDim.x;
             left = blk_tile(t, a, s_grp, tl);
+            if (left) sp = group_span(a, tl.g);
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -364,11 +524,13 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
     const uint32_t tq = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
     uint32_t it = 0;
     int parity = 0;
+    bool ok = true;
     BlkTile tl;
-    for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x, parity ^= 1) {
-      const int cnt = s_grp.cnt[tl.g];
+    for (int t = blockIdx.x; blk_tile(t, a, s_grp, tl); t += gridDim.x, parity ^= 1) {
+      const Span sp = group_span(a, tl.g);
+      const int64_t base = sp.base;
+      const int cnt = sp.cnt;
       const int row = tl.m0 + q * 32 + lane;           // within the group
-      const int64_t base = group_base(a, tl.g);
       float acc[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) acc[i] = 0.f;
@@ -376,7 +538,6 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       // TMEM buffer is handed back once the last is in, with half of the sums still to be added, and
       // the next block's first loads leave before the last chunk is added.
       uint32_t r[2][32];
-      bool ok;
       auto add = [&](int c, float f) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(r[c & 1][i]), f, acc[c * 32 + i]);
@@ -389,7 +550,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
         f0 = s_scale[it & 1][EPI == kOutSwiGLU ? 0 : half][q * 32 + lane];
         f1 = EPI == kOutSwiGLU ? s_scale[it & 1][1][q * 32 + lane] : f0;
       };
-      begin_block();
+      if (ok) begin_block();
 #pragma unroll 1
       for (int kb = 0; kb < KB && ok; ++kb) {
         const uint32_t taddr = tq + (it & 1) * kBN;
@@ -409,7 +570,11 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
         if (kb + 1 < KB) begin_block();
         add(3, f);
       }
-      if (!ok) break;
+      if (!ok) {
+        // the other half's warp of these rows may have got through: meet it at its barrier
+        if (EPI == kOutSwiGLU) asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        continue;
+      }
       // ---- output: 64 bytes of each of the warp's 32 rows at a time, through shared memory (the
       // 16-byte pieces of a row are swapped by row pair, so that 8 lanes hit distinct banks)
       const int first = tl.m0 + q * 32;
@@ -454,7 +619,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
         uint32_t top = 0;   // as bits, so that a NaN stays the largest
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
-          h[i] = __fdividef(acc[i], 1.f + __expf(-acc[i])) * acc[64 + i];
+          h[i] = silu_mul(acc[i], acc[64 + i]);
           top = max(top, __float_as_uint(fabsf(h[i])));
         }
         s_amax[parity][half][q * 32 + lane] = top;
@@ -473,8 +638,314 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       }
     }
   }
+  // Launched while the kernel for groups with few rows still runs: whoever waits for this one waits for both.
+  if (threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_before();
   __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 2 * kBN);
+  }
+}
+
+// ------------------------------------------------------------------------------- groups with few rows
+template <int EPI, bool B_MN>
+__global__ void __launch_bounds__(kBlkThreads, 1)
+    gemm_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, BlkArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* s_part = reinterpret_cast<float*>(smem + kFewStages * kFewStageBytes);   // [kFewTile][kBN] of a finished tile
+  __shared__ Groups s_grp;
+  __shared__ uint64_t ffull[kFewStages], fempty[kFewStages], ftfull[kFewBufs], ftempty[kFewBufs], pready, pfree, drain;
+  __shared__ __align__(16) float s_sa[2][64][4], s_sb[2][2][4];      // scales as they come, four K blocks a unit
+  __shared__ __align__(16) float s_scale[kFewBufs * 2 * kFewTile];   // sa * sb: [buffer][column half][row]
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int s_abort;
+
+  // The kernel for the other groups, where there is one, may take the SMs as they fall free.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = warp_id(), lane = lane_id();
+  uint32_t crank, csize;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int s = 0; s < kFewStages; ++s) {
+      mbar_init(&ffull[s], 1);
+      mbar_init(&fempty[s], 1);
+    }
+    for (int b = 0; b < kFewBufs; ++b) {
+      mbar_init(&ftfull[b], 2);   // the MMAs' commit and the scale warp
+      mbar_init(&ftempty[b], kEpiWarps);
+    }
+    mbar_init(&pready, csize);   // every CTA of the cluster has its part in shared memory
+    mbar_init(&pfree, csize);    // ... and has read this CTA's
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) tmem_alloc(&tmem_slot, 2 * kBN);
+  load_groups<true>(s_grp, a);
+  tc_fence_before();
+  __syncthreads();
+  // The peers' barriers exist once this cluster barrier completes; only the first message to a peer
+  // waits for it.
+  if (csize > 1) cluster_arrive();
+  bool joined = csize == 1;
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+  const int NB = (a.N + 127) / 128;
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.sa) | (a.sa_row * 4) | (a.sa_group * 4)) & 15) == 0;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    uint32_t it = 0;
+    FewTiles f(a, s_grp, crank, csize);
+    while (!s_abort && f.advance()) {
+      const BlkTile tl = f.tl;
+      const int row = static_cast<int>(f.sp.base) + tl.m0;
+      const int slab = a.offsets != nullptr ? 0 : tl.g;
+      // Two blocks at a time, 64 rows of one and of the other in turn: 256 contiguous bytes of each row of
+      // B are asked for together (see kFewPair).
+      for (int kb = f.k0; kb < f.k1; kb += kFewPair) {
+        const int n = min(kFewPair, f.k1 - kb);
+        bool ok = true;
+        for (int p = 0; p < n && ok; ++p)
+          ok = wait_blk(&fempty[(it + p) % kFewStages], (((it + p) / kFewStages) & 1u) ^ 1u, a, &s_abort);
+        if (!ok) break;
+        if (elect_one()) {
+          for (int p = 0; p < n; ++p) {
+            const int s = (it + p) % kFewStages;
+            mbar_arrive_expect_tx(&ffull[s], kFewStageBytes);
+            tma_load_3d(smem + s * kFewStageBytes + kBBytes, &tmA, &ffull[s], (kb + p) * kBK, row, slab);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            for (int p = 0; p < n; ++p) {
+              const int s = (it + p) % kFewStages;
+              uint8_t* db = smem + s * kFewStageBytes + j * (64 * kBK);
+              if (B_MN) tma_load_3d(db, &tmB, &ffull[s], tl.n0 + (j >> 1) * 128, (kb + p) * kBK + (j & 1) * 64, tl.g);
+              else tma_load_3d(db, &tmB, &ffull[s], (kb + p) * kBK, tl.n0 + j * 64, tl.g);
+            }
+          }
+        }
+        __syncwarp();
+        it += n;
+      }
+    }
+    if (s_abort) {  // copies in flight land before the CTA's shared memory is given up
+      for (uint32_t q = it > kFewStages ? it - kFewStages : 0; q < it; ++q)
+        mbar_wait(&ffull[q % kFewStages], (q / kFewStages) & 1u, 1000000000ull);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    uint32_t it = 0;
+    FewTiles f(a, s_grp, crank, csize);
+    while (!s_abort && f.advance()) {
+      const int n = (min(f.sp.cnt - f.tl.m0, kFewTile) + 15) / 16 * 16;
+      const uint32_t idesc = idesc_fp8(n, B_MN, false);
+      for (int kb = f.k0; kb < f.k1; ++kb, ++it) {
+        const int s = it % kFewStages, b = it % kFewBufs;
+        if (!wait_blk(&ffull[s], (it / kFewStages) & 1u, a, &s_abort)) break;
+        const uint8_t* db = smem + s * kFewStageBytes;
+        const uint64_t xd = smem_desc_k128(db + kBBytes);
+        if (!wait_blk(&ftempty[b], ((it / kFewBufs) & 1u) ^ 1u, a, &s_abort)) break;
+        tc_fence_after();
+        if (elect_one()) {
+          constexpr uint64_t wstep = B_MN ? (32 * 128) >> 4 : 2;
+          // the halves in turn: products into one accumulator wait for one another
+          const uint64_t w0 = B_MN ? smem_desc_mn128(db, 128 * kBK) : smem_desc_k128(db);
+#pragma unroll
+          for (int k = 0; k < kBK / 32; ++k) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              tc_mma_fp8(tmem_base + (b * 2 + h) * kFewCols, w0 + h * ((128 * kBK) >> 4) + wstep * k, xd + 2 * k, idesc,
+                         k > 0 ? 1u : 0u);
+          }
+          tc_commit(&ftfull[b]);
+          tc_commit(&fempty[s]);
+        }
+        __syncwarp();
+      }
+    }
+    if (elect_one()) tc_commit(&drain);  // every MMA issued is done before TMEM is released
+    __syncwarp();
+    mbar_wait(&drain, 0, a.timeout_ns);
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- scales, as in the other kernel
+    FewTiles c(a, s_grp, crank, csize);   // the unit to be copied next
+    bool left = c.advance();
+    int k0 = left ? c.k0 : 0;
+    auto copy_unit = [&](int s) {
+      if (left) {
+        const float* sa = a.sa + c.tl.g * a.sa_group + c.sp.base * a.sa_row + k0;
+#pragma unroll
+        for (int r0 = 0; r0 < kFewTile; r0 += 32)
+          if (r0 + lane < kFewTile)
+            copy_scales(s_sa[s][r0 + lane], sa + min(c.tl.m0 + r0 + lane, c.sp.cnt - 1) * a.sa_row, k0, c.k1, wide);
+        const float* sb = a.sb + c.tl.g * a.sb_group + min(c.tl.n0 / 128 + (lane >> 2 & 1), NB - 1) * a.sb_n;
+        if (lane < 8 && k0 + (lane & 3) < c.k1)
+          cp_async<4>(&s_sb[s][lane >> 2][lane & 3], sb + (k0 + (lane & 3)) * a.sb_k);
+        k0 += 4;
+        if (k0 >= c.k1) {
+          left = c.advance();
+          k0 = c.k0;
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    copy_unit(0);
+    copy_unit(1);
+    uint32_t it = 0, u = 0;
+    bool ok = true;
+    FewTiles f(a, s_grp, crank, csize);
+    while (ok && !s_abort && f.advance()) {
+      for (int kb = f.k0; kb < f.k1 && ok; ++kb, ++it) {
+        const int s = u & 1, j = (kb - f.k0) & 3, b = it % kFewBufs;
+        if (j == 0) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          __syncwarp();
+        }
+        const float b0 = s_sb[s][0][j], b1 = s_sb[s][1][j];
+        const float f0 = s_sa[s][lane][j], f1 = s_sa[s][32 + lane][j];   // (rows past kFewTile: not stored)
+        ok = wait_blk(&ftempty[b], ((it / kFewBufs) & 1u) ^ 1u, a, &s_abort);
+        float* o = s_scale + b * 2 * kFewTile + lane;
+        o[0] = f0 * b0;
+        o[kFewTile] = f0 * b1;
+        if (lane < kFewTile - 32) {
+          o[32] = f1 * b0;
+          o[kFewTile + 32] = f1 * b1;
+        }
+        __syncwarp();
+        if (lane == 0 && ok) mbar_arrive(&ftfull[b]);
+        if (j == 3 || kb + 1 == f.k1) {
+          copy_unit(s);
+          ++u;
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp >= kFirstEpi) {
+    // ---------------------------------------------------------------- epilogue
+    const int q = warp & 3, half = (warp - kFirstEpi) >> 2, ew = warp - kFirstEpi;
+    const uint32_t tq = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + half * kFewCols;
+    uint32_t it = 0, round = 0;   // round: tiles shared with the cluster so far
+    bool ok = true;
+    // (left only where bar_all says so: all eight warps, or none; whole tiles have no barrier, and pass
+    // without work once `ok` is false)
+    FewTiles ft(a, s_grp, crank, csize);
+    while (ft.advance()) {
+      const BlkTile tl = ft.tl;
+      const Span sp = ft.sp;
+      const bool split = ft.split;
+      const int n = min(sp.cnt - tl.m0, kFewTile);
+      float acc[kFewTile];
+#pragma unroll
+      for (int i = 0; i < kFewTile; ++i) acc[i] = 0.f;
+      for (int kb = ft.k0; kb < ft.k1 && ok; ++kb, ++it) {
+        const int b = it % kFewBufs;
+        ok = wait_blk(&ftfull[b], (it / kFewBufs) & 1u, a, &s_abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t taddr = tq + b * 2 * kFewCols;
+        const float4* f = reinterpret_cast<const float4*>(s_scale + (b * 2 + half) * kFewTile);
+        uint32_t r[32];
+#pragma unroll
+        for (int c = 0; c < (kFewTile + 31) / 32; ++c) {
+          if (32 * c < n) {
+            tmem_ld32(taddr + 32 * c, r);   // (columns past the rows are read and dropped)
+#pragma unroll
+            for (int i = 0; i < 8 && 32 * c + 4 * i < kFewTile; ++i) {
+              const float4 f4 = f[8 * c + i];
+              float* o = acc + 32 * c + 4 * i;
+              o[0] = fmaf(__uint_as_float(r[4 * i]), f4.x, o[0]);
+              o[1] = fmaf(__uint_as_float(r[4 * i + 1]), f4.y, o[1]);
+              o[2] = fmaf(__uint_as_float(r[4 * i + 2]), f4.z, o[2]);
+              o[3] = fmaf(__uint_as_float(r[4 * i + 3]), f4.w, o[3]);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ftempty[b]);
+      }
+      // this CTA's part, [row][256 columns], once every peer has read the one before
+      if (ok && split && round > 0) ok = wait_blk(&pfree, (round - 1) & 1u, a, &s_abort);
+      if (ok) {
+#pragma unroll
+        for (int i = 0; i < kFewTile; ++i)
+          if (i < n) s_part[i * kBN + half * 128 + q * 32 + lane] = acc[i];
+      }
+      __syncwarp();
+      if (split && !joined) {
+        cluster_wait();
+        joined = true;
+      }
+      ok = bar_all(1, 32 * kEpiWarps, ok);
+      if (!ok) break;
+      const int parts = split ? csize : 1;
+      if (split) {
+        if (ew == 0 && lane < static_cast<int>(csize)) arrive_peer(&pready, lane);
+        ok = wait_blk(&pready, round & 1u, a, &s_abort);
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+      }
+      // a warp a row, the rows divided among the CTAs with parts
+      for (int i = (split ? crank : 0) + parts * ew; ok && i < n; i += parts * kEpiWarps) {
+        const float* p = s_part + i * kBN + 4 * lane;
+        float4 x, y;
+        if (!split) {
+          x = *reinterpret_cast<const float4*>(p);
+          y = *reinterpret_cast<const float4*>(p + 128);
+        } else {
+          x = load_peer(p, 0);
+          y = load_peer(p + 128, 0);
+#pragma unroll
+          for (int c = 1; c < kMaxSplit; ++c) {   // in the order of the ranks
+            if (c < static_cast<int>(csize)) {
+              const float4 v = load_peer(p, c), w = load_peer(p + 128, c);
+              x.x += v.x, x.y += v.y, x.z += v.z, x.w += v.w;
+              y.x += w.x, y.y += w.y, y.z += w.z, y.w += w.w;
+            }
+          }
+        }
+        const int64_t grow = sp.base + tl.m0 + i;
+        const int c0 = tl.n0 + 4 * lane, c1 = c0 + 128;
+        uint8_t* crow = a.C + tl.g * a.c_group + grow * a.c_row;
+        if (EPI == kOutF32) {
+          if (c0 < a.N) *reinterpret_cast<float4*>(crow + 4ll * c0) = x;
+          if (c1 < a.N) *reinterpret_cast<float4*>(crow + 4ll * c1) = y;
+        } else if (EPI == kOutBF16 || a.C != nullptr) {
+          if (c0 < a.N) *reinterpret_cast<uint2*>(crow + 2ll * c0) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+          if (c1 < a.N) *reinterpret_cast<uint2*>(crow + 2ll * c1) = make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
+        }
+        if (EPI == kOutSwiGLU) {
+          const float h0 = silu_mul(x.x, y.x), h1 = silu_mul(x.y, y.y), h2 = silu_mul(x.z, y.z), h3 = silu_mul(x.w, y.w);
+          uint32_t top = max(max(__float_as_uint(fabsf(h0)), __float_as_uint(fabsf(h1))),
+                             max(__float_as_uint(fabsf(h2)), __float_as_uint(fabsf(h3))));
+          top = max(__reduce_max_sync(0xffffffffu, top), __float_as_uint(1e-4f));
+          const float amax = __uint_as_float(top), inv = __fdiv_rn(448.f, amax);
+          uint8_t* hrow = a.H + tl.g * a.h_group + grow * a.h_row + tl.n0 / 2;
+          reinterpret_cast<uint32_t*>(hrow)[lane] = uint32_t(f32x2_to_e4m3x2(h0 * inv, h1 * inv)) |
+                                                    (uint32_t(f32x2_to_e4m3x2(h2 * inv, h3 * inv)) << 16);
+          if (lane == 0) a.Hs[tl.g * a.hs_group + grow * a.hs_row + tl.n0 / 256] = __fdiv_rn(amax, 448.f);
+        }
+      }
+      ok = bar_all(1, 32 * kEpiWarps, ok);
+      if (!ok) break;
+      if (split) {
+        if (ew == 0 && lane < static_cast<int>(csize)) arrive_peer(&pfree, lane);
+        ++round;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (csize > 1) {   // no CTA leaves while a peer may still read its part
+    if (!joined) cluster_wait();
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 2 * kBN);
@@ -498,14 +969,85 @@ CUtensorMap map_u8_3d(const void* base, int64_t d0, int64_t d1, int64_t d2, int6
   return m;
 }
 
+// The kernel for groups with few rows in clusters of `split`; grid 0: the CTAs that are resident together
+// (a GPC's SMs need not divide into clusters) is asked for, once for each size.
 template <int EPI, bool B_MN>
-void launch_block(const CUtensorMap& ma, const CUtensorMap& mb, const BlkArgs& a, int grid, cudaStream_t stream) {
+int few_launch(const CUtensorMap& ma, const CUtensorMap& mb, const BlkArgs& a, int grid, int split, cudaStream_t stream) {
+  constexpr int smem = 1024 + kFewStages * kFewStageBytes + kFewTile * kBN * 4;
+  auto kfn = gemm_few_kernel<EPI, B_MN>;
+  static std::atomic<uint64_t> seen{0};
+  AT_CUDA_CHECK(set_smem_limit_once(seen, kfn, smem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid > 0 ? grid : split);
+  cfg.blockDim = dim3(kBlkThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = split;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = split > 1 ? 1 : 0;
+  if (grid == 0) {
+    if (split == 1) return a.sms;
+    static std::atomic<int> resident[kMaxSplit + 1] = {};
+    int clusters = resident[split].load(std::memory_order_relaxed);
+    if (clusters == 0) {
+      AT_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, kfn, &cfg));
+      TORCH_CHECK(clusters > 0, "no cluster of the fp8 GEMM fits on this device");
+      resident[split].store(clusters, std::memory_order_relaxed);
+    }
+    return std::max(1, std::min(clusters, a.sms / split)) * split;
+  }
+  AT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kfn, ma, mb, a));
+  return grid;
+}
+
+// One call: the forms that its rows take, and the launches. `rows_known`: the rows of all groups together
+// (an upper bound), or 0 where only the device knows (slabs).
+template <int EPI, bool B_MN>
+void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMap& mb, const CUtensorMap& mbf,
+                  BlkArgs a, int64_t rows_known,
+                  cudaStream_t stream) {
+  const int64_t ntn = (a.N + kBN - 1) / kBN, KB = (a.K + kBK - 1) / kBK;
+  // tiles of groups with few rows: one a group (slabs), or as many as the rows make
+  const int64_t some = std::min<int64_t>(a.G, rows_known);
+  const int64_t few = (rows_known == 0 ? a.G : std::max<int64_t>(some, (rows_known + kFewTile - 1) / kFewTile)) * ntn;
+  int64_t least = -1;
+  for (int s = 1; s <= kMaxSplit && s * 2 <= std::max<int64_t>(KB, 2) && s <= a.sms; s *= 2) {
+    const int grid = few_launch<EPI, B_MN>(ma, mb, a, 0, s, stream);
+    const int64_t cycles = few_cycles(few, KB, grid, s);
+    if (least < 0 || cycles < least) {
+      least = cycles;
+      a.split = s;
+      a.few_grid = grid;
+    }
+  }
+  if (rows_known > 0) {
+    // half a tile more a group than its rows fill, on average, and at least one
+    const int64_t many = std::max<int64_t>(some, (rows_known + kBM - 1) / kBM + some / 2) * ntn;
+    a.form = least < many_cycles(many, KB, a.sms, many == some * ntn) ? kAllFew : kAllMany;
+  } else {
+    // a decoding step, a tile a group, decides whether the form for few rows is worth its launch
+    a.form = least >= many_cycles(few, KB, a.sms, true) ? kAllMany : a.rows <= kFewTile ? kAllFew : kBothForms;
+  }
+  if (a.form != kAllMany) few_launch<EPI, B_MN>(mf, mbf, a, a.few_grid, a.split, stream);
+  if (a.form == kAllFew) return;
   constexpr int smem = 1024 + kStages * kStageBytes + kEpiWarps * kWarpStage;
   auto kfn = gemm_block_kernel<EPI, B_MN>;
   static std::atomic<uint64_t> seen{0};
   AT_CUDA_CHECK(set_smem_limit_once(seen, kfn, smem));
-  kfn<<<grid, kBlkThreads, smem, stream>>>(ma, mb, a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.sms);
+  cfg.blockDim = dim3(kBlkThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = a.form == kBothForms ? 1 : 0;
+  AT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kfn, ma, mb, a));
 }
 
 bool on(const at::Tensor& t, const at::Tensor& like) { return t.device() == like.device(); }
@@ -590,6 +1132,9 @@ void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at:
     a.c_row = C->stride(-2) * C->element_size();
     a.c_group = masked ? C->stride(0) * C->element_size() : 0;
   }
+  const int64_t most_tiles = ((masked ? int64_t(a.G) * ((a.rows + kFewTile - 1) / kFewTile) : a.rows / kFewTile + a.G)) *
+                             ((N + kBN - 1) / kBN);
+  TORCH_CHECK(most_tiles < (1ll << 30), "too many tiles");
   if (!A.is_cuda() || a.rows == 0) return;  // CPU tensors: the checks alone
   const c10::cuda::CUDAGuard guard(A.device());
   TORCH_CHECK(on(error, A) && error.scalar_type() == at::kInt, "error word");
@@ -607,16 +1152,21 @@ void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at:
   const int64_t s1 = stride(A, A.dim() - 2, K);
   const CUtensorMap ma = masked ? map_u8_3d(A.data_ptr(), K, a.rows, a.G, s1, stride(A, 0, s1 * a.rows), kBM)
                                 : map_u8_3d(A.data_ptr(), K, a.rows, 1, s1, s1 * a.rows, kBM);
+  const CUtensorMap mf = masked ? map_u8_3d(A.data_ptr(), K, a.rows, a.G, s1, stride(A, 0, s1 * a.rows), kFewTile)
+                                : map_u8_3d(A.data_ptr(), K, a.rows, 1, s1, s1 * a.rows, kFewTile);
   const CUtensorMap mb = b_kn ? map_u8_3d(B.data_ptr(), N, K, a.G, N, N * K, kBK)
                               : map_u8_3d(B.data_ptr(), K, N, a.G, K, N * K, kBN);
-  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int grid = num_sms > 0 ? static_cast<int>(std::min<int64_t>(num_sms, sms)) : sms;
+  const CUtensorMap mbf = b_kn ? map_u8_3d(B.data_ptr(), N, K, a.G, N, N * K, 64)
+                               : map_u8_3d(B.data_ptr(), K, N, a.G, K, N * K, 64);
+  const int all = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  a.sms = num_sms > 0 ? static_cast<int>(std::min<int64_t>(num_sms, all)) : all;
+  const int64_t known = masked ? 0 : a.rows;
   auto stream = at::cuda::getCurrentCUDAStream();
-  if (epilogue == kOutSwiGLU) launch_block<kOutSwiGLU, false>(ma, mb, a, grid, stream);
-  else if (epilogue == kOutBF16 && b_kn) launch_block<kOutBF16, true>(ma, mb, a, grid, stream);
-  else if (epilogue == kOutBF16) launch_block<kOutBF16, false>(ma, mb, a, grid, stream);
-  else if (b_kn) launch_block<kOutF32, true>(ma, mb, a, grid, stream);
-  else launch_block<kOutF32, false>(ma, mb, a, grid, stream);
+  if (epilogue == kOutSwiGLU) launch_block<kOutSwiGLU, false>(ma, mf, mb, mbf, a, known, stream);
+  else if (epilogue == kOutBF16 && b_kn) launch_block<kOutBF16, true>(ma, mf, mb, mbf, a, known, stream);
+  else if (epilogue == kOutBF16) launch_block<kOutBF16, false>(ma, mf, mb, mbf, a, known, stream);
+  else if (b_kn) launch_block<kOutF32, true>(ma, mf, mb, mbf, a, known, stream);
+  else launch_block<kOutF32, false>(ma, mf, mb, mbf, a, known, stream);
 }
 
 }  // namespace b200ep

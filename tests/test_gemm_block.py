@@ -161,12 +161,42 @@ def test_block_long_reduction(epilogue, kn):
 
 @pytest.mark.gpu
 @needs_cuda
+@pytest.mark.parametrize('epilogue,kn,N', [('bf16', False, 264), ('swiglu', False, 1024), ('f32', True, 272),
+                                          ('f32', False, 2560)])
+@pytest.mark.parametrize('counts', [[1], [64], [65, 3], [300], [17, 0, 64, 90]])
+def test_block_few_rows_divide_k(counts, epilogue, kn, N):
+    # few tiles: clusters divide K (19 blocks, so that the shares differ and end inside a scale unit)
+    _segment_case(counts, N, 2320, epilogue, kn, 'cuda', seed=N)
+
+
+@pytest.mark.gpu
+@needs_cuda
+@pytest.mark.parametrize('epilogue,G,N,K,num_sms', [
+    ('bf16', 3, 768, 2048, 8), ('swiglu', 5, 1024, 1920, 8), ('f32', 9, 256, 7168, 16),   # clusters, several rounds
+    ('swiglu', 17, 2560, 2048, 0), ('bf16', 40, 2560, 1024, 0)])
+def test_block_few_rows_many_rounds(epilogue, G, N, K, num_sms):
+    # slabs of a decoding step: every CTA or cluster works through several tiles
+    g = torch.Generator().manual_seed(N)
+    counts = torch.randint(0, 50, (G,), generator=g).tolist()
+    _masked_case(counts, 64, N, K, epilogue, 'cuda', seed=N, num_sms=num_sms, pre=G % 2 == 0)
+
+
+@pytest.mark.gpu
+@needs_cuda
+@pytest.mark.parametrize('epilogue', ['bf16', 'swiglu'])
+def test_block_both_forms_in_one_call(epilogue):
+    # groups with few and with many rows, more tiles than SMs of each
+    _segment_case([1, 400, 64, 0, 65, 1100, 30, 512, 7] * 4, 1280, 400, epilogue, False, 'cuda', seed=6, head=2, tail=3)
+
+
+@pytest.mark.gpu
+@needs_cuda
 def test_block_many_groups():
     _segment_case([i % 4 for i in range(1024)], 64, 128, 'f32', False, 'cuda', seed=4)
     _segment_case([3, 0, 200, 64] * 40, 128, 256, 'bf16', True, 'cuda', seed=5)
 
 
-def _masked_case(counts, cap, N, K, epilogue, dev, strided=False, kn=False, seed=0):
+def _masked_case(counts, cap, N, K, epilogue, dev, strided=False, kn=False, seed=0, num_sms=0, pre=True):
     g = torch.Generator().manual_seed(seed)
     G = len(counts)
     q, sc = _rows((G, cap), K, g)
@@ -187,19 +217,21 @@ def _masked_case(counts, cap, N, K, epilogue, dev, strided=False, kn=False, seed
         kw = dict(out=torch.full((G, cap, N), 7.0, dtype=torch.bfloat16, device=dev))
     if epilogue == 'swiglu':
         kw.update(h_out=torch.full((G, cap, N // 2), 0x11, dtype=torch.uint8, device=dev).view(F8),
-                  h_scales=torch.full((G, cap, N // 256), 7.0, device=dev), save_preact=True)
-    res = _run(q, sc, B, sb, epilogue, kn, None, cnt, dev, **kw)
+                  h_scales=torch.full((G, cap, N // 256), 7.0, device=dev), save_preact=pre)
+    if epilogue == 'f32':
+        kw['out'] = kw['out'].float()
+    res = _run(q, sc, B, sb, epilogue, kn, None, cnt, dev, num_sms=num_sms, **kw)
     for e, n in enumerate(counts):
         n = max(0, min(n, cap))
-        pre = res[2] if epilogue == 'swiglu' else res
-        assert (pre[e, n:].float() == 7).all()
+        out = res[2] if epilogue == 'swiglu' else res
+        assert out is None or (out[e, n:].float() == 7).all()
         if epilogue == 'swiglu':
             assert (res[0].view(torch.uint8)[e, n:] == 0x11).all() and (res[1][e, n:] == 7).all()
         if n == 0:
             continue
         ref, mag = _expected(q[e:e + 1].cpu(), sc[e:e + 1].cpu(), B[e:e + 1], sb[e:e + 1], (0, slice(0, n)), 0, kn)
         if epilogue == 'swiglu':
-            _check_swiglu(res[0][e, :n], res[1][e, :n], res[2][e, :n], ref, mag, K)
+            _check_swiglu(res[0][e, :n], res[1][e, :n], None if out is None else out[e, :n], ref, mag, K)
         else:
             _check(res[e, :n], ref, mag, K)
     if strided:
