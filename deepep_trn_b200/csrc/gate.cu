@@ -12,15 +12,21 @@
 //  * without a bias, and with groups ranked by their largest value, the order of c is that of
 //    the logits themselves (both scores grow with the logit), which are compared as they are;
 //  * otherwise c is formed in fp32 with a bound on its error, and a row in which two values whose
-//    order matters lie closer than that bound is selected again in fp64. With 256 experts that
-//    is a few rows in a thousand.
+//    order matters lie closer than that bound is selected again in fp64. With 256 experts, 8 of
+//    them chosen from 4 of 8 groups, that is two rows in a thousand.
 //
 // Forward and backward read each logit once (T * E) and write T * k * 12 or T * E; a warp takes
-// one token, its experts in the lanes' registers.
+// one token, its experts in the lanes' registers (16-byte loads and stores where the rows allow).
+// Values are compared as integers of the same order, so that one redux finds the warp's largest.
+// Bound by instruction issue (about 1100 a row of 256 experts, 8 groups, 8 chosen): 16384 such tokens
+// forward and backward in 40 us where their bytes would take 6 (59 us with values compared as floats by
+// shuffles, 4-byte accesses and ids looked for in every lane); one token 4.0 us (7.2 before), of which
+// 2.5 are a launch.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cfloat>
+#include <climits>
 
 #include "ops.h"
 
@@ -39,7 +45,8 @@ struct GateArgs {
   float* w;
   int T, E, K;
   int n, g, gs;          // groups, groups kept, experts per group
-  int lanes;             // lanes that scan one group (power of two, lanes * n <= 32)
+  int lanes;             // lanes that scan one group in shared memory (power of two, lanes * n <= 32)
+  int reg_lanes;         // lanes that hold one group in registers (a power of two), or 0
   int sigmoid, top2, renorm;
   float scale;
 };
@@ -59,19 +66,12 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 // A logit as the gate sees it: NaN is unavailable, +inf is the largest finite value (so that a
 // softmax stays defined), -0 is +0.
 __device__ __forceinline__ float clean_logit(float v) {
-  return v != v ? -INFINITY : fminf(v, FLT_MAX) + 0.f;
+  return fminf(fmaxf(v, -INFINITY), FLT_MAX) + 0.f;   // fmaxf drops a NaN
 }
 __device__ __forceinline__ float sigmoid_f32(float x) {
   const float e = expf(-fabsf(x));
   return (x >= 0.f ? 1.f : e) / (1.f + e);
 }
-
-template <typename T>
-__device__ __forceinline__ T low();
-template <>
-__device__ __forceinline__ float low<float>() { return -INFINITY; }
-template <>
-__device__ __forceinline__ double low<double>() { return -static_cast<double>(INFINITY); }
 
 template <typename T>
 __device__ __forceinline__ T warp_max(T v) {
@@ -89,59 +89,133 @@ __device__ __forceinline__ T warp_sum(T v) {
   return v;
 }
 
-// Selection over the warp's values v (lane holds experts lane * EPT + i), destroying them:
-// lane j < K gets the j-th largest's id in `mine` (-1 where nothing is left). `slack(a)` bounds
-// how far apart two values near `a` must be for their order to be certain; false is returned if
-// some order that matters is not. `buf`: E + lanes * n values of shared memory of this warp.
-template <typename T, int EPT, typename Slack>
-__device__ __forceinline__ bool select(const GateArgs& a, T (&v)[EPT], T* buf, int lane, int& mine, Slack slack) {
-  bool sure = true;
-  if (a.n > 1) {
-    // group values: `lanes` lanes scan each group through shared memory (a group is skewed by
-    // `lanes` words from the one before, so that the lanes of different groups hit other banks)
+// Integers in the order of the floats (no NaN, no -0).
+__device__ __forceinline__ int key_of(float v) {
+  const int b = __float_as_int(v);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float of_key(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+constexpr int kNone = static_cast<int>(0x807fffffu);   // key_of(-inf): nothing, or unavailable
+
+// EPT consecutive values of a row from `row`, as fp32 (-inf past E).
+template <typename T, int EPT, bool VEC>
+__device__ __forceinline__ void load_row(float (&l)[EPT], const T* __restrict__ row, int first, int E) {
+  if constexpr (VEC) {
+    constexpr int kPer = 16 / sizeof(T) < EPT ? 16 / sizeof(T) : EPT;   // values a load
+#pragma unroll
+    for (int i = 0; i < EPT; i += kPer) {
+      alignas(16) T t[kPer];
+      if (first + i < E) {   // E is a multiple of kPer
+        if constexpr (kPer * sizeof(T) == 16) *reinterpret_cast<int4*>(t) = *reinterpret_cast<const int4*>(row + first + i);
+        else if constexpr (kPer * sizeof(T) == 8) *reinterpret_cast<int2*>(t) = *reinterpret_cast<const int2*>(row + first + i);
+        else if constexpr (kPer * sizeof(T) == 4) *reinterpret_cast<int*>(t) = *reinterpret_cast<const int*>(row + first + i);
+        else t[0] = row[first + i];
+      }
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) l[i + j] = first + i < E ? to_f32(t[j]) : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) l[i] = first + i < E ? to_f32(row[first + i]) : -INFINITY;
+  }
+}
+template <typename T, int EPT, bool VEC>
+__device__ __forceinline__ void store_row(T* __restrict__ row, const float (&l)[EPT], int first, int E) {
+  if constexpr (VEC) {
+    constexpr int kPer = 16 / sizeof(T) < EPT ? 16 / sizeof(T) : EPT;
+#pragma unroll
+    for (int i = 0; i < EPT; i += kPer) {
+      alignas(16) T t[kPer];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) t[j] = from_f32<T>(l[i + j]);
+      if (first + i < E) {
+        if constexpr (kPer * sizeof(T) == 16) *reinterpret_cast<int4*>(row + first + i) = *reinterpret_cast<const int4*>(t);
+        else if constexpr (kPer * sizeof(T) == 8) *reinterpret_cast<int2*>(row + first + i) = *reinterpret_cast<const int2*>(t);
+        else if constexpr (kPer * sizeof(T) == 4) *reinterpret_cast<int*>(row + first + i) = *reinterpret_cast<const int*>(t);
+        else row[first + i] = t[0];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+      if (first + i < E) row[first + i] = from_f32<T>(l[i]);
+  }
+}
+
+// The groups' part of the selection: of the warp's keys v (lane holds experts lane * EPT + i) those of
+// the groups that are not kept become kNone. k0 (if not 0) bounds the error of one score; to it come the
+// roundings of the bias's and the groups' sums, two units of 2^-24 of a value. False is returned if some
+// order that matters is not certain.
+template <int EPT>
+__device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], int* buf, int lane, float k0) {
+  int t0 = kNone, t1 = kNone;   // the two largest of the group that this lane helps to scan
+  const int lanes = a.reg_lanes > 0 ? a.reg_lanes : a.lanes, shift = __ffs(lanes) - 1;
+  if (a.reg_lanes > 0) {
+    // a group is the experts of `reg_lanes` whole lanes
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      t1 = max(t1, min(t0, v[i]));
+      t0 = max(t0, v[i]);
+    }
+  } else {
+    // through shared memory, `lanes` lanes a group (a group is skewed by `lanes` words from the one
+    // before, so that the lanes of different groups hit other banks)
+    int grp = lane * EPT / a.gs, left = a.gs - (lane * EPT - grp * a.gs);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       const int e = lane * EPT + i;
-      if (e < a.E) buf[e + e / a.gs * a.lanes] = v[i];
-    }
-    __syncwarp();
-    const int grp = lane / a.lanes, sub = lane % a.lanes;
-    T t0 = low<T>(), t1 = low<T>();
-    if (grp < a.n) {
-      const T* p = buf + grp * (a.gs + a.lanes);
-      for (int j = sub; j < a.gs; j += a.lanes) {
-        const T x = p[j];
-        if (x > t0) {
-          t1 = t0;
-          t0 = x;
-        } else if (x > t1) {
-          t1 = x;
-        }
+      if (e < a.E) buf[e + grp * lanes] = v[i];
+      if (--left == 0) {
+        ++grp;
+        left = a.gs;
       }
     }
-    for (int m = a.lanes >> 1; m >= 1; m >>= 1) {
-      const T o0 = __shfl_xor_sync(kAll, t0, m), o1 = __shfl_xor_sync(kAll, t1, m);
-      const T hi = o0 > t0 ? o0 : t0, lo = o0 > t0 ? t0 : o0;
-      const T s = o1 > t1 ? o1 : t1;
-      t0 = hi;
-      t1 = lo > s ? lo : s;
+    __syncwarp();
+    const int g = lane >> shift, sub = lane & (lanes - 1);
+    if (g < a.n) {
+      const int* p = buf + g * (a.gs + lanes);
+      for (int j = sub; j < a.gs; j += lanes) {
+        t1 = max(t1, min(t0, p[j]));
+        t0 = max(t0, p[j]);
+      }
     }
-    // the sum counts the second value only where there is one
-    const T gv = grp >= a.n ? low<T>() : (a.top2 && t1 > low<T>() ? t0 + t1 : t0);
-    int rank = 0;
-    for (int j = 0; j < a.n; ++j) {
-      const T o = __shfl_sync(kAll, gv, j * a.lanes);
-      rank += (o > gv || (o == gv && j < grp)) ? 1 : 0;
+  }
+  for (int m = lanes >> 1; m >= 1; m >>= 1) {
+    const int o0 = __shfl_xor_sync(kAll, t0, m), o1 = __shfl_xor_sync(kAll, t1, m);
+    t1 = max(min(t0, o0), max(t1, o1));
+    t0 = max(t0, o0);
+  }
+  // the sum counts the second value only where there is one
+  const int grp = lane >> shift;
+  int gv = grp >= a.n ? kNone : a.top2 && t1 > kNone ? key_of(of_key(t0) + of_key(t1) + 0.f) : t0;
+  bool in = false;
+  int worst_in = INT_MAX;
+#pragma unroll 1
+  for (int j = 0; j < a.g; ++j) {   // the best group left; its lanes hold the same value, ties go to the first
+    const int top = __reduce_max_sync(kAll, gv);
+    if (top == kNone) break;
+    const int from = (__ffs(__ballot_sync(kAll, gv == top)) - 1) >> shift;
+    if (grp == from) {
+      in = true;
+      gv = kNone;
     }
-    const bool in = grp < a.n && rank < a.g && gv > low<T>();
+    worst_in = top;
+  }
+  bool sure = true;
+  if (k0 > 0.f) {
+    const int best_out = __reduce_max_sync(kAll, gv);
+    const float x = of_key(worst_in), y = of_key(best_out);
+    sure = best_out == kNone || x - y > 4.f * k0 + (fabsf(x) + fabsf(y)) * 0x1p-22f;
+  }
+  if (a.reg_lanes > 0) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) v[i] = in ? v[i] : kNone;
+  } else {
     const uint32_t kept = __ballot_sync(kAll, in);
-    const T worst_in = -warp_max(in ? -gv : low<T>());
-    const T best_out = warp_max(in ? low<T>() : gv);
-    if (best_out > low<T>() && !(worst_in - best_out > slack(worst_in) + slack(best_out))) sure = false;
-    int of = lane * EPT / a.gs, left = a.gs - lane * EPT % a.gs;
+    int of = lane * EPT / a.gs, left = a.gs - (lane * EPT - of * a.gs);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      if (of >= a.n || !((kept >> (of * a.lanes & 31)) & 1u)) v[i] = low<T>();
+      if (of >= a.n || !((kept >> ((of << shift) & 31)) & 1u)) v[i] = kNone;
       if (--left == 0) {
         ++of;
         left = a.gs;
@@ -149,64 +223,164 @@ __device__ __forceinline__ bool select(const GateArgs& a, T (&v)[EPT], T* buf, i
     }
     __syncwarp();
   }
-  mine = -1;
-  T before = low<T>();
-  for (int k = 0; k <= a.K; ++k) {
-    T best = low<T>();
-    int at = 0;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) {
-      if (v[i] > best) {
-        best = v[i];
-        at = i;
-      }
-    }
-    const T top = warp_max(best);
-    if (top == low<T>()) break;
-    if (k > 0 && !(before - top > slack(before))) sure = false;
-    if (k == a.K) break;
-    before = top;
-    const int from = __ffs(__ballot_sync(kAll, best == top)) - 1;  // ids grow with the lane
-    const int id = __shfl_sync(kAll, lane * EPT + at, from);
-    if (lane == k) mine = id;
-    if (lane == from) {
-#pragma unroll
-      for (int i = 0; i < EPT; ++i)
-        if (i == at) v[i] = low<T>();
-    }
-  }
   return sure;
 }
 
-// The same selection with scores in fp64.
+// PACKED: the low bits of a key hold EPT - 1 - i, so that a key names its place in the lane and the lower
+// id of two equal values comes first. The bits are free where the values are 16-bit logits, and below
+// the values' certainty where scores are compared.
 template <int EPT>
-__device__ __noinline__ int select_f64(const GateArgs& a, const float* l, double* buf, int lane) {
-  double v[EPT];
-  double top = 0, sum = 1;
+constexpr int kPackMask = EPT == 1 ? 0 : EPT == 2 ? 1 : EPT == 4 ? 3 : EPT == 8 ? 7 : EPT == 16 ? 15 : 31;
+
+// The K largest keys in order: lane j < K gets the j-th one's id in `mine` (-1 where nothing is left).
+template <int EPT, bool PACKED>
+__device__ __forceinline__ bool take_largest(const GateArgs& a, int (&v)[EPT], int lane, float k0, int& mine) {
+  constexpr int M = kPackMask<EPT>;
+  bool sure = true;
+  if constexpr (PACKED) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) v[i] = v[i] == kNone ? INT_MIN : (v[i] & ~M) | (M - i);
+    if constexpr (EPT <= 8) {   // each lane's keys in descending order: bubbles of compare and exchange
+#pragma unroll
+      for (int i = EPT - 1; i > 0; --i)
+#pragma unroll
+        for (int j = 0; j < i; ++j) {
+          const int hi = max(v[j], v[j + 1]), lo = min(v[j], v[j + 1]);
+          v[j] = hi;
+          v[j + 1] = lo;
+        }
+    }
+  }
+  constexpr int kLow = PACKED ? INT_MIN : kNone;
+  float before = 0.f;
+  int best = kLow, key = kLow, lane_of = 0;   // lane k: the k-th key and its lane
+  if constexpr (PACKED && EPT <= 8) {
+    best = v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) best = max(best, v[i]);
+  }
+  int at = 0;
+  const int rounds = k0 > 0.f ? a.K + 1 : a.K;   // one more for the distance of the last from the first left out
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    // without the places, which order equal values within a lane only
+    const int value = PACKED ? best & ~M : best;
+    const int top = __reduce_max_sync(kAll, value);
+    if (top == kLow) break;
+    if (k0 > 0.f) {
+      const float x = of_key(top);
+      // the scores' errors, the bias's roundings and the low bits that packing took
+      if (k > 0 && !(before - x > 2.f * k0 + (fabsf(before) + fabsf(x)) * (PACKED ? (M + 2) * 0x1p-23f : 0x1p-23f))) sure = false;
+      before = x;
+    }
+    if (k == a.K) break;
+    const int from = __ffs(__ballot_sync(kAll, value == top)) - 1;  // ids grow with the lane
+    const int won = PACKED ? __shfl_sync(kAll, best, from) : top;
+    if (lane == k) {
+      key = won;
+      lane_of = from;
+    }
+    if constexpr (PACKED && EPT <= 8) {
+      const bool mine_goes = lane == from;
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) v[i] = mine_goes ? (i + 1 < EPT ? v[i + 1] : INT_MIN) : v[i];
+      best = v[0];
+    } else if constexpr (PACKED) {
+      if (lane == from) {
+        best = INT_MIN;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+          v[i] = v[i] == won ? INT_MIN : v[i];
+          best = max(best, v[i]);
+        }
+      }
+    } else {
+      int p = 0;
+      if (lane == from) {
+        best = kNone;
+        bool gone = false;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+          if (!gone && v[i] == top) {
+            p = i;
+            v[i] = kNone;
+            gone = true;
+          }
+          best = max(best, v[i]);
+        }
+      }
+      p = __shfl_sync(kAll, p, from);
+      if (lane == k) at = p;
+    }
+  }
+  mine = key == kLow ? -1 : lane_of * EPT + (PACKED ? M - (key & M) : at);
+  return sure;
+}
+
+// The same selection with scores in fp64, for the rows that need it: one value of shared memory an
+// expert, every step in order.
+__device__ __noinline__ int select_f64(const GateArgs& a, const float* l, int ept, double* v, int lane) {
+  double top = -static_cast<double>(INFINITY), sum = 0;
   if (!a.sigmoid) {
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) m = fmaxf(m, l[i]);
-    top = warp_max(m);
-    sum = 0;
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) sum += l[i] > -INFINITY ? exp(static_cast<double>(l[i]) - top) : 0.0;
+    for (int i = 0; i < ept; ++i) top = fmax(top, static_cast<double>(l[i]));
+    top = warp_max(top);
+    for (int i = 0; i < ept; ++i) sum += l[i] > -INFINITY ? exp(static_cast<double>(l[i]) - top) : 0.0;
     sum = warp_sum(sum);
   }
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    const int e = lane * EPT + i;
+  const double none = -static_cast<double>(INFINITY);
+  for (int i = 0; i < ept; ++i) {
+    const int e = lane * ept + i;
+    if (e >= a.E) continue;
     const double x = l[i];
     double s = a.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x - top) / sum;
-    if (a.bias != nullptr && e < a.E) s += static_cast<double>(a.bias[e]);
-    v[i] = l[i] > -INFINITY && s == s ? s : low<double>();
+    if (a.bias != nullptr) s += static_cast<double>(a.bias[e]);
+    v[e] = l[i] > -INFINITY && s == s ? s : none;
   }
-  int mine;
-  select<double, EPT>(a, v, buf, lane, mine, [](double) { return 0.0; });
+  __syncwarp();
+  if (a.n > 1) {
+    double t0 = none, t1 = none;   // lane j: group j
+    for (int j = 0; lane < a.n && j < a.gs; ++j) {
+      const double x = v[lane * a.gs + j];
+      if (x > t0) {
+        t1 = t0;
+        t0 = x;
+      } else if (x > t1) {
+        t1 = x;
+      }
+    }
+    const double gv = a.top2 && t1 > none ? t0 + t1 : t0;
+    int rank = 0;
+    for (int j = 0; j < a.n; ++j) {
+      const double o = __shfl_sync(kAll, gv, j);
+      rank += (o > gv || (o == gv && j < lane)) ? 1 : 0;
+    }
+    const uint32_t kept = __ballot_sync(kAll, lane < a.n && rank < a.g && gv > none);
+    for (int e = lane; e < a.E; e += 32)
+      if (!((kept >> (e / a.gs)) & 1u)) v[e] = none;
+    __syncwarp();
+  }
+  int mine = -1;
+  for (int k = 0; k < a.K; ++k) {
+    double best = none;
+    int at = INT_MAX;
+    for (int e = lane; e < a.E; e += 32)
+      if (v[e] > best) {
+        best = v[e];
+        at = e;
+      }
+    const double top_v = warp_max(best);
+    if (top_v == none) break;
+    const int id = __reduce_min_sync(kAll, best == top_v ? at : INT_MAX);
+    if (lane == k) mine = id;
+    __syncwarp();
+    if (lane == 0) v[id] = none;
+    __syncwarp();
+  }
   return mine;
 }
 
-template <typename T, int EPT>
+template <typename T, int EPT, bool VEC>
 __global__ void __launch_bounds__(kGateWarps * 32) gate_kernel(GateArgs a) {
   extern __shared__ double gate_smem[];
   const int lane = lane_id(), warp = warp_id();
@@ -214,48 +388,51 @@ __global__ void __launch_bounds__(kGateWarps * 32) gate_kernel(GateArgs a) {
   if (t >= a.T) return;  // whole warps only: no barrier follows
   double* buf = gate_smem + static_cast<int64_t>(warp) * (a.E + 32);
   const T* row = static_cast<const T*>(a.logits) + static_cast<int64_t>(t) * a.stride;
-  float l[EPT], v[EPT];
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    const int e = lane * EPT + i;
-    l[i] = e < a.E ? clean_logit(to_f32(row[e])) : -INFINITY;
-  }
-  float m = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) m = fmaxf(m, l[i]);
-  m = warp_max(m);
+  float l[EPT];
+  load_row<T, EPT, VEC>(l, row, lane * EPT, a.E);
   const bool direct = a.bias == nullptr && (a.n == 1 || !a.top2);
-  int mine;
-  float sum = 1.f;
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) l[i] = clean_logit(l[i]);
+  float m = 0.f, sum = 1.f;
   if (!a.sigmoid && !(direct && a.renorm)) {
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) m = fmaxf(m, l[i]);
+    m = of_key(__reduce_max_sync(kAll, key_of(m)));
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) sum += l[i] > -INFINITY ? expf(l[i] - m) : 0.f;
+    for (int i = 0; i < EPT; ++i) sum += l[i] > -INFINITY ? __expf(l[i] - m) : 0.f;
     sum = warp_sum(sum);
   }
+  int v[EPT];
+  float k0 = 0.f;
   if (direct) {
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) v[i] = l[i];
-    select<float, EPT>(a, v, reinterpret_cast<float*>(buf), lane, mine, [](float) { return 0.f; });
+    for (int i = 0; i < EPT; ++i) v[i] = key_of(l[i]);
   } else {
-    const float inv = 1.f / sum;
+    const float inv = __fdividef(1.f, sum);
+    float bias[EPT];
+    if (a.bias != nullptr) load_row<float, EPT, VEC>(bias, a.bias, lane * EPT, a.E);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      const int e = lane * EPT + i;
-      const float s = a.sigmoid ? sigmoid_f32(l[i]) : expf(l[i] - m) * inv;
-      const float c = a.bias != nullptr && e < a.E ? s + a.bias[e] : s;
-      v[i] = l[i] > -INFINITY && c == c ? c + 0.f : -INFINITY;
+      const float x = __expf(a.sigmoid ? -l[i] : l[i] - m);
+      float c = a.sigmoid ? __fdividef(1.f, 1.f + x) : x * inv;
+      if (a.bias != nullptr) c = fmaxf(c + bias[i], -INFINITY);   // (a NaN is dropped)
+      v[i] = l[i] > -INFINITY ? key_of(c + 0.f) : kNone;
     }
-    // Each score is within 2^-21 of its value relative to itself (an exponential and a division
-    // within 2 units each, the sums within 1), so within 2^-21 * (largest score); the bias adds
-    // one rounding of the sum, and a sum of two such values doubles both and adds another. The
-    // bounds below are twice that, for one value of a pair.
-    const float most = a.sigmoid ? 1.f : inv;
-    const float k0 = most * 0x1p-18f;
-    const bool sure = select<float, EPT>(a, v, reinterpret_cast<float*>(buf), lane, mine,
-                                         [k0](float x) { return k0 + fabsf(x) * 0x1p-21f; });
-    if (!sure) mine = select_f64<EPT>(a, l, buf, lane);
+    // Bound of one score's error, k0. With the documented errors of __expf (2 + 1.173 |x| units of 2^-23)
+    // and __fdividef (2 units):  sigmoid: s (1 - s) (2 + 1.173 |x|) + 1/2 + 2 < 3.3 units, so 2^-20;
+    // softmax, relative to the largest score: 3 units each for the exponential and the sum's terms, 18
+    // for adding up to 1024 of them, 2 for the quotient: 26 units, so 2^-18.
+    k0 = a.sigmoid ? 0x1p-20f : inv * 0x1p-18f;
   }
+  bool sure = true;
+  if (a.n > 1) sure = keep_groups<EPT>(a, v, reinterpret_cast<int*>(buf), lane, k0);
+  int mine;
+  // packed keys: 16-bit logits end in 16 zero bits as fp32, and scores are certain to 2^-18 at best
+  const bool packed = sizeof(T) == 2 || !direct;
+  if (!(packed ? take_largest<EPT, true>(a, v, lane, k0, mine) : take_largest<EPT, false>(a, v, lane, k0, mine))) sure = false;
+  if (!sure) mine = select_f64(a, l, EPT, buf, lane);
   // weights from the logits of the chosen
   const float x = mine >= 0 ? clean_logit(to_f32(row[mine])) : -INFINITY;
   const bool has = mine >= 0;
@@ -263,7 +440,7 @@ __global__ void __launch_bounds__(kGateWarps * 32) gate_kernel(GateArgs a) {
   if (a.renorm) {
     // both scores are proportional to exp(x - r) times a factor between 1/2 and 1 (sigmoid) or 1;
     // r keeps the sum from underflowing
-    const float top = warp_max(x);
+    const float top = of_key(__reduce_max_sync(kAll, key_of(x)));
     if (a.sigmoid) {
       const float r = fminf(top, 0.f);
       w = !has ? 0.f : (x >= 0.f ? 1.f / (1.f + expf(-x)) : expf(x - r) / (1.f + expf(x)));
@@ -298,8 +475,9 @@ struct GateBwdArgs {
 //   softmax, renorm  d_k = p_k (dw_k - sum_j p_j dw_j)      (the softmax over the chosen)
 //   softmax          d_e = p_e ([e chosen] dw_e - sum_j p_j dw_j)   for every e of the row
 // zero elsewhere. An id that occurs twice gets the sum; ids outside [0, E) count for nothing.
-template <typename T, int EPT>
+template <typename T, int EPT, bool VEC>
 __global__ void __launch_bounds__(kGateWarps * 32) gate_bwd_kernel(GateBwdArgs a) {
+  extern __shared__ float gate_bwd_smem[];
   const int lane = lane_id(), warp = warp_id();
   const int t = blockIdx.x * kGateWarps + warp;
   if (t >= a.T) return;
@@ -321,17 +499,17 @@ __global__ void __launch_bounds__(kGateWarps * 32) gate_bwd_kernel(GateBwdArgs a
   const bool whole = !a.sigmoid && !a.renorm;
   if (whole) {
     m = -INFINITY;
+    load_row<T, EPT, VEC>(l, row, lane * EPT, a.E);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      const int e = lane * EPT + i;
-      l[i] = e < a.E ? clean_logit(to_f32(row[e])) : -INFINITY;
+      l[i] = clean_logit(l[i]);
       m = fmaxf(m, l[i]);
     }
     m = warp_max(m);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      l[i] = l[i] > -INFINITY ? expf(l[i] - m) : 0.f;
+      l[i] = l[i] > -INFINITY ? __expf(l[i] - m) : 0.f;
       sum += l[i];
     }
     sum = warp_sum(sum);
@@ -354,51 +532,81 @@ __global__ void __launch_bounds__(kGateWarps * 32) gate_bwd_kernel(GateBwdArgs a
     dot = warp_sum(p * dw);
     gk = has ? p * (dw - dot) * (a.sigmoid ? sigmoid_f32(-x) : 1.f) : 0.f;
   }
+  // the chosen experts' values into the row: through shared memory, or one by one where an id occurs twice
   float out[EPT];
+  const uint32_t same = __match_any_sync(kAll, id >= 0 ? id : -1 - lane);
+  if (__all_sync(kAll, (same & (same - 1)) == 0)) {
+    float* buf = gate_bwd_smem + warp * 32 * EPT;
 #pragma unroll
-  for (int i = 0; i < EPT; ++i) out[i] = 0.f;
-  for (int k = 0; k < a.K; ++k) {
-    const int e = __shfl_sync(kAll, id, k);
-    const float g = __shfl_sync(kAll, gk, k);
+    for (int i = 0; i < EPT; ++i) buf[i * 32 + lane] = 0.f;
+    __syncwarp();
+    // expert e lies at [e % EPT][e / EPT], so that the lanes read their own without bank conflicts
+    if (id >= 0) buf[id % EPT * 32 + id / EPT] = gk;
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < EPT; ++i)
-      if (e == lane * EPT + i) out[i] += g;
+    for (int i = 0; i < EPT; ++i) out[i] = buf[i * 32 + lane];
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) out[i] = 0.f;
+    for (int k = 0; k < a.K; ++k) {
+      const int e = __shfl_sync(kAll, id, k);
+      const float g = __shfl_sync(kAll, gk, k);
+#pragma unroll
+      for (int i = 0; i < EPT; ++i)
+        if (e == lane * EPT + i) out[i] += g;
+    }
   }
   if (whole) {
 #pragma unroll
     for (int i = 0; i < EPT; ++i) out[i] = l[i] * inv * (out[i] - dot);
   }
-  T* drow = static_cast<T*>(a.d) + static_cast<int64_t>(t) * a.E;
-#pragma unroll
-  for (int i = 0; i < EPT; ++i) {
-    const int e = lane * EPT + i;
-    if (e < a.E) drow[e] = from_f32<T>(out[i]);
-  }
+  store_row<T, EPT, VEC>(static_cast<T*>(a.d) + static_cast<int64_t>(t) * a.E, out, lane * EPT, a.E);
 }
 
+// Whether rows of `ept` values a lane can be moved in the widest words that hold them.
+template <typename T>
+bool rows_align(const void* p, int64_t stride, int E, int ept) {
+  const int64_t per = std::min<int64_t>(16 / sizeof(T), ept), bytes = per * sizeof(T);
+  return E % per == 0 && reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * static_cast<int64_t>(sizeof(T)) % bytes == 0;
+}
+
+template <typename T, int EPT>
+void launch_gate_ept(GateArgs a, cudaStream_t s) {
+  const int grid = (a.T + kGateWarps - 1) / kGateWarps;
+  const size_t smem = sizeof(double) * kGateWarps * (a.E + 32);
+  const int lanes = a.gs / EPT;
+  a.reg_lanes = a.gs % EPT == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+  if (rows_align<T>(a.logits, a.stride, a.E, EPT) && (a.bias == nullptr || rows_align<float>(a.bias, a.E, a.E, EPT)))
+    gate_kernel<T, EPT, true><<<grid, kGateWarps * 32, smem, s>>>(a);
+  else gate_kernel<T, EPT, false><<<grid, kGateWarps * 32, smem, s>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+template <typename T, int EPT>
+void launch_gate_bwd_ept(const GateBwdArgs& a, cudaStream_t s) {
+  const int grid = (a.T + kGateWarps - 1) / kGateWarps;
+  const size_t smem = sizeof(float) * kGateWarps * 32 * EPT;
+  if (rows_align<T>(a.logits, a.stride, a.E, EPT) && rows_align<T>(a.d, a.E, a.E, EPT))
+    gate_bwd_kernel<T, EPT, true><<<grid, kGateWarps * 32, smem, s>>>(a);
+  else gate_bwd_kernel<T, EPT, false><<<grid, kGateWarps * 32, smem, s>>>(a);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
 template <typename T>
 void launch_gate(const GateArgs& a, cudaStream_t s) {
-  const int grid = (a.T + kGateWarps - 1) / kGateWarps;
-  const size_t smem = a.n > 1 ? sizeof(double) * kGateWarps * (a.E + 32) : 0;
-  if (a.E <= 32) gate_kernel<T, 1><<<grid, kGateWarps * 32, smem, s>>>(a);
-  else if (a.E <= 64) gate_kernel<T, 2><<<grid, kGateWarps * 32, smem, s>>>(a);
-  else if (a.E <= 128) gate_kernel<T, 4><<<grid, kGateWarps * 32, smem, s>>>(a);
-  else if (a.E <= 256) gate_kernel<T, 8><<<grid, kGateWarps * 32, smem, s>>>(a);
-  else if (a.E <= 512) gate_kernel<T, 16><<<grid, kGateWarps * 32, smem, s>>>(a);
-  else gate_kernel<T, 32><<<grid, kGateWarps * 32, smem, s>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (a.E <= 32) launch_gate_ept<T, 1>(a, s);
+  else if (a.E <= 64) launch_gate_ept<T, 2>(a, s);
+  else if (a.E <= 128) launch_gate_ept<T, 4>(a, s);
+  else if (a.E <= 256) launch_gate_ept<T, 8>(a, s);
+  else if (a.E <= 512) launch_gate_ept<T, 16>(a, s);
+  else launch_gate_ept<T, 32>(a, s);
 }
-
 template <typename T>
 void launch_gate_bwd(const GateBwdArgs& a, cudaStream_t s) {
-  const int grid = (a.T + kGateWarps - 1) / kGateWarps;
-  if (a.E <= 32) gate_bwd_kernel<T, 1><<<grid, kGateWarps * 32, 0, s>>>(a);
-  else if (a.E <= 64) gate_bwd_kernel<T, 2><<<grid, kGateWarps * 32, 0, s>>>(a);
-  else if (a.E <= 128) gate_bwd_kernel<T, 4><<<grid, kGateWarps * 32, 0, s>>>(a);
-  else if (a.E <= 256) gate_bwd_kernel<T, 8><<<grid, kGateWarps * 32, 0, s>>>(a);
-  else if (a.E <= 512) gate_bwd_kernel<T, 16><<<grid, kGateWarps * 32, 0, s>>>(a);
-  else gate_bwd_kernel<T, 32><<<grid, kGateWarps * 32, 0, s>>>(a);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (a.E <= 32) launch_gate_bwd_ept<T, 1>(a, s);
+  else if (a.E <= 64) launch_gate_bwd_ept<T, 2>(a, s);
+  else if (a.E <= 128) launch_gate_bwd_ept<T, 4>(a, s);
+  else if (a.E <= 256) launch_gate_bwd_ept<T, 8>(a, s);
+  else if (a.E <= 512) launch_gate_bwd_ept<T, 16>(a, s);
+  else launch_gate_bwd_ept<T, 32>(a, s);
 }
 
 void check_logits(const at::Tensor& logits) {
