@@ -16,6 +16,13 @@ Weights: W1 [EL, 2I, H] with gate and up rows interleaved in 128-row blocks
 (``ops.gemm.interleave_gate_up``), W2 [EL, H, I], router Wr [E, H]; all bf16.
 Router logits come out of the same tensor-core GEMM with an fp32 epilogue, so
 expert selection matches an fp32 router up to summation order.
+
+``gate`` replaces the softmax over the chosen k by ``ops.moe_ops.router_gate`` (sigmoid or softmax
+scores, expert groups, renormalisation, scale; ``router_bias`` then steers the selection only).
+``fp8_block`` runs dispatch and the experts' products in e4m3 with fp32 scales, 1x128 for rows and
+128x128 for weights, in training and inference: SwiGLU's result leaves the first product quantised, the
+input gradients read the same weights the other way round, the weight gradients stay bf16.
+``forward_low_latency`` is its generation step over the low-latency dispatch and combine.
 """
 from __future__ import annotations
 
@@ -24,7 +31,7 @@ import torch.nn as nn
 
 from ..ops import gemm as G
 from ..ops import moe_ops as MO
-from ..ops.quant import quantize_fp8
+from ..ops.quant import dequantize_fp8, quantize_fp8
 from ..utils.profiling import timer
 
 
@@ -51,15 +58,39 @@ def _expert_forward(rows, offsets, W1, W2):
     return h, pre, o
 
 
+def _route(logits, topk, router_bias, gate):
+    """(ids, weights): the chosen-k softmax of the biased logits, or ``router_gate``."""
+    if gate is None:
+        return MO.router_topk(logits if router_bias is None else logits + router_bias, topk)
+    return MO.router_gate(logits, topk, bias=router_bias, **gate)
+
+
+def _route_bwd(logits, idx, w, dw, num_experts, gate):
+    if gate is None:
+        return MO.router_topk_bwd(idx, w, dw.float(), num_experts)
+    kw = {k: gate[k] for k in ('scoring', 'renormalize', 'scale') if k in gate}
+    return MO.router_gate_bwd(logits, idx, dw, **kw)
+
+
+def _router_grads(ctx, x, Wr, logits, idx, w, dw, dx):
+    """(dx + dlogits @ Wr, dWr): summed in fp32 in the GEMM's epilogue, one rounding."""
+    dlogits = _route_bwd(logits, idx, w, dw, ctx.num_experts, ctx.gate).to(x.dtype)
+    seg = _single_segment(x.shape[0], x.device)
+    dx = G.grouped_gemm(dlogits, Wr.unsqueeze(0), seg, b_layout='kn', residual=dx.contiguous())
+    if ctx.num_experts % 64 == 0:
+        dWr = G.grouped_gemm_wgrad(dlogits, x, seg, out_dtype=Wr.dtype)[0]            # [E, H]
+    else:  # the token-major operand path tiles M in 64-wide atoms
+        dWr = G.grouped_gemm_wgrad(MO.transpose(dlogits), MO.transpose(x), seg, out_dtype=Wr.dtype, layout='mk')[0]
+    return dx, dWr
+
+
 class _MoEFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, Wr, W1, W2, buf, num_experts, topk, router_bias=None, fp8_dispatch=False):
+    def forward(ctx, x, Wr, W1, W2, buf, num_experts, topk, router_bias=None, fp8_dispatch=False, gate=None):
         EL = num_experts // buf.group_size
         with timer.stage('moe.router'):
             logits = router_logits(x, Wr)
-            if router_bias is not None:
-                logits = logits + router_bias
-            idx, w = MO.router_topk(logits, topk)
+            idx, w = _route(logits, topk, router_bias, gate)
         with timer.stage('moe.dispatch'):
             ntr, _, nte, itr, _ = buf.get_dispatch_layout(idx, num_experts)
             # fp8_dispatch: tokens travel as e4m3 with 1x128 scales (quantised inside the
@@ -74,13 +105,14 @@ class _MoEFunction(torch.autograd.Function):
         with timer.stage('moe.combine'):
             # the weighted un-permute (sum_k w * o[pos]) is formed inside the combine kernel
             y, _, _ = buf.combine(o, handle, pair_pos=pos, pair_weights=recv_w)
-        ctx.save_for_backward(x, Wr, W1, W2, idx, w, recv_w, pos, offsets, counts, rows, pre, h, o)
-        ctx.buf, ctx.handle, ctx.num_experts = buf, handle, num_experts
+        ctx.save_for_backward(x, Wr, W1, W2, logits if gate is not None else None, idx, w, recv_w, pos, offsets, counts,
+                              rows, pre, h, o)
+        ctx.buf, ctx.handle, ctx.num_experts, ctx.gate = buf, handle, num_experts, gate
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, Wr, W1, W2, idx, w, recv_w, pos, offsets, counts, rows, pre, h, o = ctx.saved_tensors
+        x, Wr, W1, W2, logits, idx, w, recv_w, pos, offsets, counts, rows, pre, h, o = ctx.saved_tensors
         buf, handle = ctx.buf, ctx.handle
         dy = dy.contiguous().to(x.dtype)
         with timer.stage('moe.bwd.dispatch'):
@@ -101,16 +133,63 @@ class _MoEFunction(torch.autograd.Function):
         with timer.stage('moe.bwd.combine'):
             dx, dw, _ = buf.combine(d_recv_x, handle, topk_weights=d_recv_w)   # dispatch backward
         with timer.stage('moe.bwd.router'):
-            dlogits = MO.router_topk_bwd(idx, w, dw.float(), ctx.num_experts).to(x.dtype)
-            seg = _single_segment(x.shape[0], x.device)
-            # dx = combine's dx + dlogits @ Wr, summed in fp32 in the GEMM epilogue, one rounding
-            dx = G.grouped_gemm(dlogits, Wr.unsqueeze(0), seg, b_layout='kn', residual=dx.contiguous())
-            if ctx.num_experts % 64 == 0:
-                dWr = G.grouped_gemm_wgrad(dlogits, x, seg, out_dtype=Wr.dtype)[0]            # [E, H]
-            else:  # the token-major operand path tiles M in 64-wide atoms
-                dWr = G.grouped_gemm_wgrad(MO.transpose(dlogits), MO.transpose(x), seg, out_dtype=Wr.dtype,
-                                           layout='mk')[0]
-        return dx, dWr, dW1, dW2, None, None, None, None, None
+            dx, dWr = _router_grads(ctx, x, Wr, logits, idx, w, dw, dx)
+        return dx, dWr, dW1, dW2, None, None, None, None, None, None
+
+
+class _MoEBlockFunction(torch.autograd.Function):
+    """The layer with e4m3 rows and weights and fp32 block scales. ``wq``: the quantised weights
+    (q1, s1, q2, s2) of W1 and W2; the gradients go to W1 and W2 themselves."""
+
+    @staticmethod
+    def forward(ctx, x, Wr, W1, W2, wq, buf, num_experts, topk, router_bias, gate, train):
+        EL = num_experts // buf.group_size
+        q1, s1, q2, s2 = wq
+        with timer.stage('moe.router'):
+            logits = router_logits(x, Wr)
+            idx, w = _route(logits, topk, router_bias, gate)
+        with timer.stage('moe.dispatch'):
+            ntr, _, nte, itr, _ = buf.get_dispatch_layout(idx, num_experts)
+            recv_x, recv_idx, recv_w, per_expert, handle, _ = buf.dispatch(
+                x, topk_idx=idx, topk_weights=w, num_tokens_per_rank=ntr, is_token_in_rank=itr,
+                num_tokens_per_expert=nte, use_fp8=True)
+        with timer.stage('moe.permute'):
+            (rq, rs), pos, offsets, counts = MO.permute(recv_x, recv_idx, EL, per_expert, keep_fp8=True)
+        with timer.stage('moe.experts'):
+            h, hs, pre = G.grouped_gemm_fp8_block(rq, rs, q1, s1, offsets, epilogue='swiglu', save_preact=train)
+            o = G.grouped_gemm_fp8_block(h, hs, q2, s2, offsets)
+        with timer.stage('moe.combine'):
+            y, _, _ = buf.combine(o, handle, pair_pos=pos, pair_weights=recv_w)
+        if train:
+            ctx.save_for_backward(x, Wr, q1, s1, q2, s2, logits if gate is not None else None, idx, w, recv_w, pos,
+                                  offsets, counts, rq, rs, pre, h, hs, o)
+            ctx.buf, ctx.handle, ctx.num_experts, ctx.gate = buf, handle, num_experts, gate
+            ctx.w_dtypes = W1.dtype, W2.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        (x, Wr, q1, s1, q2, s2, logits, idx, w, recv_w, pos, offsets, counts, rq, rs, pre, h, hs, o) = ctx.saved_tensors
+        buf, handle = ctx.buf, ctx.handle
+        dy = dy.contiguous().to(x.dtype)
+        with timer.stage('moe.bwd.dispatch'):
+            dy_recv, *_ = buf.dispatch(dy, handle=handle)                  # combine backward
+        with timer.stage('moe.bwd.unpermute'):
+            d_o, d_recv_w = MO.unpermute_bwd(dy_recv, o, pos, recv_w, offsets, counts)
+        with timer.stage('moe.bwd.dgrad'):
+            dh = G.grouped_gemm_fp8_block(*quantize_fp8(d_o), q2, s2, offsets, b_layout='kn')        # d_o @ W2[e]
+            dpre = MO.swiglu_bwd(dh, pre)
+            drows = G.grouped_gemm_fp8_block(*quantize_fp8(dpre), q1, s1, offsets, b_layout='kn')    # dpre @ W1[e]
+        with timer.stage('moe.bwd.wgrad'):
+            dW2 = G.grouped_gemm_wgrad(d_o, dequantize_fp8(h, hs), offsets, out_dtype=ctx.w_dtypes[1])
+            dW1 = G.grouped_gemm_wgrad(dpre, dequantize_fp8(rq, rs), offsets, out_dtype=ctx.w_dtypes[0])
+        with timer.stage('moe.bwd.permute'):
+            d_recv_x = MO.permute_bwd(drows, pos)
+        with timer.stage('moe.bwd.combine'):
+            dx, dw, _ = buf.combine(d_recv_x, handle, topk_weights=d_recv_w)   # dispatch backward
+        with timer.stage('moe.bwd.router'):
+            dx, dWr = _router_grads(ctx, x, Wr, logits, idx, w, dw, dx)
+        return dx, dWr, dW1, dW2, None, None, None, None, None, None, None
 
 
 class MoELayer(nn.Module):
@@ -118,7 +197,8 @@ class MoELayer(nn.Module):
 
     def __init__(self, buffer, hidden: int, intermediate: int, num_experts: int, topk: int,
                  dtype=torch.bfloat16, device=None, init_std: float = 0.02, seed: int = 0,
-                 fp8_dispatch: bool = False, fp8_experts: bool = False):
+                 fp8_dispatch: bool = False, fp8_experts: bool = False, gate: dict | None = None,
+                 fp8_block: bool = False):
         super().__init__()
         R = buffer.group_size
         if num_experts % R:
@@ -129,6 +209,12 @@ class MoELayer(nn.Module):
         self.fp8_dispatch = fp8_dispatch   # forward tokens cross NVLink as fp8 e4m3 + 1x128 scales
         # inference (no autograd): fp8 dispatch and block-scaled fp8 expert GEMMs on e4m3 weights
         self.fp8_experts = fp8_experts
+        if fp8_experts and (fp8_block or gate is not None):
+            raise ValueError('fp8_experts (power-of-two scales) takes neither fp8_block nor gate')
+        # keyword arguments of router_gate (scoring, num_groups, topk_groups, group_score, renormalize, scale)
+        self.gate = dict(gate) if gate is not None else None
+        # e4m3 dispatch and experts with fp32 block scales, in training too
+        self.fp8_block = fp8_block
         self._fp8_cache = None
         self.hidden, self.intermediate = hidden, intermediate
         self.num_experts, self.topk = num_experts, topk
@@ -147,8 +233,9 @@ class MoELayer(nn.Module):
         self.w1 = nn.Parameter(G.interleave_gate_up(wg, wu))
         del wg, wu
         self.w2 = nn.Parameter(randn(EL, hidden, intermediate, gen=g_local))
-        # fp32 bias added to the router logits before top-k (not trained here; it steers load,
-        # e.g. a Zipf skew for benchmarks or a balancing bias)
+        # fp32 bias added to the router logits before top-k, or with `gate` to its scores for the
+        # selection only (not trained here; it steers load, e.g. a Zipf skew for benchmarks or a
+        # balancing bias)
         self.register_buffer('router_bias', torch.zeros(num_experts, dtype=torch.float32, device=device))
 
     def _fp8_weights(self):
@@ -166,6 +253,32 @@ class MoELayer(nn.Module):
                 q2, s2 = G.quantize_fp8_blocks(self.w2)
                 self._fp8_cache = (key, q1, G.fp8_scale_tiles(s1, EL), q2, G.fp8_scale_tiles(s2, EL))
         return self._fp8_cache[1:]
+
+    def _block_weights(self):
+        """(q1, s1, q2, s2): e4m3 expert weights with 128x128 fp32 scales, rebuilt when the weights change."""
+        key = (self.w1._version, self.w2._version, self.w1.data_ptr(), self.w2.data_ptr())
+        if self._fp8_cache is None or self._fp8_cache[0] != key:
+            with torch.no_grad():
+                self._fp8_cache = (key, *G.quantize_fp8_weight(self.w1), *G.quantize_fp8_weight(self.w2))
+        return self._fp8_cache[1:]
+
+    @torch.no_grad()
+    def forward_low_latency(self, x: torch.Tensor, num_max_tokens_per_rank: int) -> torch.Tensor:
+        """A generation step (``fp8_block`` layers): low-latency dispatch -> expert slabs -> combine. ``x`` holds
+        at most ``num_max_tokens_per_rank`` tokens, which all ranks give alike. Nothing waits on the host, so
+        the step can be captured into a CUDA graph after one call."""
+        if not self.fp8_block:
+            raise ValueError('forward_low_latency needs fp8_block=True')
+        q1, s1, q2, s2 = self._block_weights()
+        with timer.stage('moe.router'):
+            idx, w = _route(router_logits(x, self.router), self.topk, self.router_bias, self.gate)
+        (rq, rs), counts, handle, _, _ = self.buffer.low_latency_dispatch(x, idx, num_max_tokens_per_rank,
+                                                                          self.num_experts, use_fp8=True)
+        with timer.stage('moe.experts'):
+            h, hs, _ = G.grouped_gemm_fp8_block(rq, rs, q1, s1, counts=counts, epilogue='swiglu')
+            o = G.grouped_gemm_fp8_block(h, hs, q2, s2, counts=counts)
+        y, _, _ = self.buffer.low_latency_combine(o, idx, w, handle)
+        return y
 
     def _forward_fp8(self, x: torch.Tensor) -> torch.Tensor:
         buf, E = self.buffer, self.num_experts
@@ -193,8 +306,12 @@ class MoELayer(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.fp8_experts and not torch.is_grad_enabled():
             return self._forward_fp8(x)
+        if self.fp8_block:
+            return _MoEBlockFunction.apply(x, self.router, self.w1, self.w2, self._block_weights(), self.buffer,
+                                           self.num_experts, self.topk, self.router_bias, self.gate,
+                                           torch.is_grad_enabled())
         return _MoEFunction.apply(x, self.router, self.w1, self.w2, self.buffer, self.num_experts, self.topk,
-                                  self.router_bias, self.fp8_dispatch)
+                                  self.router_bias, self.fp8_dispatch, self.gate)
 
 
 def reference_moe(x, Wr, W1, W2, topk, router_bias=None):

@@ -45,6 +45,33 @@ def _(idx, w, dw, num_experts):
     return w.new_empty(w.shape[0], num_experts, dtype=torch.float32)
 
 
+@torch.library.custom_op(f'{_LIB}::router_gate', mutates_args=())
+def router_gate(logits: torch.Tensor, k: int, scoring: str = 'sigmoid', bias: torch.Tensor | None = None,
+                num_groups: int = 1, topk_groups: int = 1, group_score: str = 'top2', renormalize: bool = True,
+                scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Expert ids (int64, -1 where nothing is left) and weights (fp32) of the grouped gate."""
+    return _MO.router_gate(logits, k, scoring, bias, num_groups, topk_groups, group_score, renormalize, scale)
+
+
+@router_gate.register_fake
+def _(logits, k, scoring='sigmoid', bias=None, num_groups=1, topk_groups=1, group_score='top2', renormalize=True,
+      scale=1.0):
+    T = logits.shape[0]
+    return logits.new_empty(T, k, dtype=torch.int64), logits.new_empty(T, k, dtype=torch.float32)
+
+
+@torch.library.custom_op(f'{_LIB}::router_gate_bwd', mutates_args=())
+def router_gate_bwd(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, scoring: str = 'sigmoid',
+                    renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of the gate's weights w.r.t. the logits (their type)."""
+    return _MO.router_gate_bwd(logits, idx, dw, scoring, renormalize, scale)
+
+
+@router_gate_bwd.register_fake
+def _(logits, idx, dw, scoring='sigmoid', renormalize=True, scale=1.0):
+    return logits.new_empty(logits.shape)
+
+
 @torch.library.custom_op(f'{_LIB}::permute', mutates_args=())
 def permute(x: torch.Tensor, local_ids: torch.Tensor, num_local_experts: int) -> tuple[
         torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -133,5 +160,50 @@ def _(A, B, offsets, out_dtype=torch.bfloat16):
     return A.new_empty(offsets.shape[0] - 1, A.shape[1], B.shape[1], dtype=out_dtype)
 
 
+@torch.library.custom_op(f'{_LIB}::quantize_fp8_weight', mutates_args=())
+def quantize_fp8_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """e4m3 weights with one fp32 scale per 128 x 128 block."""
+    return _G.quantize_fp8_weight(w)
+
+
+@quantize_fp8_weight.register_fake
+def _(w):
+    *lead, N, K = w.shape
+    return (w.new_empty(w.shape, dtype=torch.float8_e4m3fn),
+            w.new_empty(*lead, (N + 127) // 128, (K + 127) // 128, dtype=torch.float32))
+
+
+@torch.library.custom_op(f'{_LIB}::grouped_gemm_fp8_block', mutates_args=())
+def grouped_gemm_fp8_block(A: torch.Tensor, sa: torch.Tensor, B: torch.Tensor, sb: torch.Tensor,
+                           offsets: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                           epilogue: str = 'bf16', b_layout: str = 'nk') -> torch.Tensor:
+    """fp8 products with 1x128 row and 128x128 weight scales, bf16 or fp32 output."""
+    if epilogue == 'swiglu':
+        raise ValueError('use grouped_gemm_fp8_swiglu')
+    return _G.grouped_gemm_fp8_block(A, sa, B, sb, offsets, counts, epilogue=epilogue, b_layout=b_layout)
+
+
+@grouped_gemm_fp8_block.register_fake
+def _(A, sa, B, sb, offsets=None, counts=None, epilogue='bf16', b_layout='nk'):
+    N = B.shape[2] if b_layout == 'kn' else B.shape[1]
+    return A.new_empty(*A.shape[:-1], N, dtype=torch.float32 if epilogue == 'f32' else torch.bfloat16)
+
+
+@torch.library.custom_op(f'{_LIB}::grouped_gemm_fp8_swiglu', mutates_args=())
+def grouped_gemm_fp8_swiglu(A: torch.Tensor, sa: torch.Tensor, B: torch.Tensor, sb: torch.Tensor,
+                            offsets: torch.Tensor | None = None,
+                            counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(h e4m3, its 1x128 scales, bf16 pre-activation) of the first expert product."""
+    return _G.grouped_gemm_fp8_block(A, sa, B, sb, offsets, counts, epilogue='swiglu', save_preact=True)
+
+
+@grouped_gemm_fp8_swiglu.register_fake
+def _(A, sa, B, sb, offsets=None, counts=None):
+    lead, N = A.shape[:-1], B.shape[1]
+    return (A.new_empty(*lead, N // 2, dtype=torch.float8_e4m3fn), A.new_empty(*lead, N // 256, dtype=torch.float32),
+            A.new_empty(*lead, N, dtype=torch.bfloat16))
+
+
 __all__ = ['router_topk', 'router_topk_bwd', 'permute', 'unpermute', 'permute_bwd', 'swiglu_bwd', 'quantize_fp8',
-           'grouped_gemm', 'grouped_gemm_wgrad']
+           'grouped_gemm', 'grouped_gemm_wgrad', 'router_gate', 'router_gate_bwd', 'quantize_fp8_weight',
+           'grouped_gemm_fp8_block', 'grouped_gemm_fp8_swiglu']
