@@ -23,6 +23,7 @@
 // shuffles, 4-byte accesses and ids looked for in every lane); one token 4.0 us (7.2 before), of which
 // 2.5 are a launch.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <cfloat>
@@ -46,6 +47,7 @@ struct GateArgs {
   int T, E, K;
   int n, g, gs;          // groups, groups kept, experts per group
   int lanes;             // lanes that scan one group in shared memory (power of two, lanes * n <= 32)
+  float inv_gs;          // 1 / gs
   int reg_lanes;         // lanes that hold one group in registers (a power of two), or 0
   int sigmoid, top2, renorm;
   float scale;
@@ -142,6 +144,9 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const float (&l)[
   }
 }
 
+// e / gs for e <= 1024: a half more than e is never within a rounding of a multiple of gs.
+__device__ __forceinline__ int group_of(const GateArgs& a, int e) { return static_cast<int>((e + 0.5f) * a.inv_gs); }
+
 // The groups' part of the selection: of the warp's keys v (lane holds experts lane * EPT + i) those of
 // the groups that are not kept become kNone. k0 (if not 0) bounds the error of one score; to it come the
 // roundings of the bias's and the groups' sums, two units of 2^-24 of a value. False is returned if some
@@ -160,7 +165,7 @@ __device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], in
   } else {
     // through shared memory, `lanes` lanes a group (a group is skewed by `lanes` words from the one
     // before, so that the lanes of different groups hit other banks)
-    int grp = lane * EPT / a.gs, left = a.gs - (lane * EPT - grp * a.gs);
+    int grp = group_of(a, lane * EPT), left = a.gs - (lane * EPT - grp * a.gs);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       const int e = lane * EPT + i;
@@ -212,7 +217,7 @@ __device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], in
     for (int i = 0; i < EPT; ++i) v[i] = in ? v[i] : kNone;
   } else {
     const uint32_t kept = __ballot_sync(kAll, in);
-    int of = lane * EPT / a.gs, left = a.gs - (lane * EPT - of * a.gs);
+    int of = group_of(a, lane * EPT), left = a.gs - (lane * EPT - of * a.gs);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
       if (of >= a.n || !((kept >> ((of << shift) & 31)) & 1u)) v[i] = kNone;
@@ -638,6 +643,7 @@ std::tuple<at::Tensor, at::Tensor> router_gate(const at::Tensor& logits, int64_t
   a.n = static_cast<int>(num_groups);
   a.g = static_cast<int>(topk_groups);
   a.gs = a.E / a.n;
+  a.inv_gs = 1.f / a.gs;
   a.lanes = 32;
   while (a.lanes * a.n > 32) a.lanes >>= 1;
   if (bias.has_value()) {
@@ -648,8 +654,8 @@ std::tuple<at::Tensor, at::Tensor> router_gate(const at::Tensor& logits, int64_t
   }
   if (!logits.is_cuda()) return {};  // the checks alone
   const c10::cuda::CUDAGuard guard(logits.device());
-  auto idx = at::empty({a.T, a.K}, logits.options().dtype(at::kLong));
-  auto w = at::empty({a.T, a.K}, logits.options().dtype(at::kFloat));
+  at::Tensor idx = at::detail::empty_cuda({a.T, a.K}, at::kLong, logits.device(), c10::nullopt);
+  at::Tensor w = at::detail::empty_cuda({a.T, a.K}, at::kFloat, logits.device(), c10::nullopt);
   if (a.T == 0) return {idx, w};
   a.logits = logits.data_ptr();
   a.stride = logits.stride(0);
@@ -680,7 +686,7 @@ at::Tensor router_gate_bwd(const at::Tensor& logits, const at::Tensor& idx, cons
               "dw must be contiguous fp32 [T, k]");
   if (!logits.is_cuda()) return {};  // the checks alone
   const c10::cuda::CUDAGuard guard(logits.device());
-  auto d = at::empty({a.T, a.E}, logits.options());
+  at::Tensor d = at::detail::empty_cuda({a.T, a.E}, logits.scalar_type(), logits.device(), c10::nullopt);
   if (a.T == 0) return d;
   a.K = static_cast<int>(idx.size(1));
   a.logits = logits.data_ptr();

@@ -898,17 +898,27 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
           x = *reinterpret_cast<const float4*>(p);
           y = *reinterpret_cast<const float4*>(p + 128);
         } else {
-          x = load_peer(p, 0);
-          y = load_peer(p + 128, 0);
+            x = y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int c = 1; c < kMaxSplit; ++c) {   // in the order of the ranks
-            if (c < static_cast<int>(csize)) {
-              const float4 v = load_peer(p, c), w = load_peer(p + 128, c);
-              x.x += v.x, x.y += v.y, x.z += v.z, x.w += v.w;
-              y.x += w.x, y.y += w.y, y.z += w.z, y.w += w.w;
+            for (int c0 = 0; c0 < kMaxSplit; c0 += 4) {   // in the order of the ranks, four on their way at a time
+              if (c0 < static_cast<int>(csize)) {
+                float4 v[4], w[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const int from = min(c0 + c, static_cast<int>(csize) - 1);
+                  v[c] = load_peer(p, from);
+                  w[c] = load_peer(p + 128, from);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  if (c0 + c < static_cast<int>(csize)) {
+                    x.x += v[c].x, x.y += v[c].y, x.z += v[c].z, x.w += v[c].w;
+                    y.x += w[c].x, y.y += w[c].y, y.z += w[c].z, y.w += w[c].w;
+                  }
+                }
+              }
             }
           }
-        }
         const int64_t grow = sp.base + tl.m0 + i;
         const int c0 = tl.n0 + 4 * lane, c1 = c0 + 128;
         uint8_t* crow = a.C + tl.g * a.c_group + grow * a.c_row;

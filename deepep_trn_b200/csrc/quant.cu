@@ -1,6 +1,7 @@
 // N6: standalone per-token, per-128-channel e4m3 quantisation (the same
 // device function the dispatch kernels fuse into their send path).
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "ops.h"
@@ -187,10 +188,10 @@ std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w) {
   TORCH_CHECK(N < (1 << 30) && K < (1 << 30), "sizes below 2^30");
   const int64_t NB = (N + 127) / 128, KB = (K + 127) / 128;
   auto shape = w.sizes().vec();
-  auto q = at::empty(shape, w.options().dtype(at::kByte));
+  at::Tensor q = at::detail::empty_cuda(shape, at::kFloat8_e4m3fn, w.device(), c10::nullopt);
   shape[shape.size() - 2] = NB;
   shape.back() = KB;
-  auto sc = at::empty(shape, w.options().dtype(at::kFloat));
+  at::Tensor sc = at::detail::empty_cuda(shape, at::kFloat, w.device(), c10::nullopt);
   const int64_t blocks = G * NB * KB;
   if (blocks == 0) return {q, sc};
   TORCH_CHECK(blocks < (1ll << 31), "too many blocks");
@@ -202,7 +203,7 @@ std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w) {
     using T = decltype(zero);
     auto k = vec ? quant_weight_kernel<T, true> : quant_weight_kernel<T, false>;
     k<<<static_cast<unsigned>(blocks), kWqThreads, 0, s>>>(static_cast<const T*>(w.data_ptr()), row, group,
-                                                          q.data_ptr<uint8_t>(), sc.data_ptr<float>(),
+                                                          static_cast<uint8_t*>(q.data_ptr()), sc.data_ptr<float>(),
                                                           static_cast<int>(N), static_cast<int>(K),
                                                           static_cast<int>(NB), static_cast<int>(KB));
   };

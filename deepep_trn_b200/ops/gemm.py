@@ -132,8 +132,7 @@ def quantize_fp8_weight(w: torch.Tensor):
         if available():
             load().quant_fp8_weight(w)   # the argument checks
         return quantize_fp8_128x128(w)
-    q, sc = load().quant_fp8_weight(w)
-    return q.view(torch.float8_e4m3fn), sc
+    return load().quant_fp8_weight(w)
 
 
 def grouped_gemm_fp8_block(A, sa, B, sb, offsets=None, counts=None, out=None, epilogue: str = 'bf16',
