@@ -71,7 +71,7 @@ enum Form : int { kBothForms = 0, kAllMany = 1, kAllFew = 2 };
 enum BlkEpilogue : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiGLU = 2 };
 
 // Estimated cycles, from measurements. A K block of a tile takes 900, or 1540 where all SMs read a part of
-// B of their own from memory. A tile with few rows costs 2300 more, and 16000 where a cluster divides K.
+// B of their own from memory. A tile with few rows costs 2300 more, and 6000 where a cluster divides K.
 // (Decoding, 32 groups of 32 rows: N 4096, K 7168, 512 tiles: 181 us as many rows, in 4 rounds, 165 as
 // few; N 7168, K 2048, 896 tiles: 91 and 100 us. One row, N 2048, K 7168: 14 and 10.7 us.)
 __host__ __device__ inline int64_t block_cycles(int64_t ctas, int64_t sms, bool own) { return own && ctas * 2 > sms ? 1540 : 900; }
@@ -82,7 +82,7 @@ __host__ __device__ inline int64_t few_cycles(int64_t tiles, int64_t KB, int64_t
   if (split == 1) return (tiles + grid - 1) / grid * (KB * block_cycles(tiles, grid, true) + 2300) + 4000;
   const int64_t left = tiles % grid, rounds = (left * split + grid - 1) / grid;
   return tiles / grid * (KB * 1540 + 2300) +
-         rounds * ((KB + split - 1) / split * block_cycles(left * split, grid, true) + 16000) + 4000;
+         rounds * ((KB + split - 1) / split * block_cycles(left * split, grid, true) + 6000) + 4000;
 }
 
 struct BlkArgs {
@@ -1034,9 +1034,11 @@ void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMa
     }
   }
   if (rows_known > 0) {
+    a.few_grid = static_cast<int>(std::min<int64_t>(a.few_grid, few * a.split));   // no CTA without work
     // half a tile more a group than its rows fill, on average, and at least one
     const int64_t many = std::max<int64_t>(some, (rows_known + kBM - 1) / kBM + some / 2) * ntn;
     a.form = least < many_cycles(many, KB, a.sms, many == some * ntn) ? kAllFew : kAllMany;
+    a.sms = static_cast<int>(std::min<int64_t>(a.sms, many));
   } else {
     // a decoding step, a tile a group, decides whether the form for few rows is worth its launch
     a.form = least >= many_cycles(few, KB, a.sms, true) ? kAllMany : a.rows <= kFewTile ? kAllFew : kBothForms;
