@@ -18,9 +18,9 @@
 // Forward and backward read each logit once (T * E) and write T * k * 12 or T * E; a warp takes
 // one token, its experts in the lanes' registers (16-byte loads and stores where the rows allow).
 // Values are compared as integers of the same order, so that one redux finds the warp's largest.
-// Bound by instruction issue (about 1100 a row of 256 experts, 8 groups, 8 chosen): 16384 such tokens
-// forward and backward in 40 us where their bytes would take 6 (59 us with values compared as floats by
-// shuffles, 4-byte accesses and ids looked for in every lane); one token 4.0 us (7.2 before), of which
+// Bound by instruction issue (about 1000 a row of 256 experts, 8 groups, 8 chosen): 16384 such tokens
+// forward and backward in 38 us where their bytes would take 6 (59 us with values compared as floats by
+// shuffles, 4-byte accesses and ids looked for in every lane); one token 3.9 us (7.2 before), of which
 // 2.5 are a launch.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -241,7 +241,6 @@ constexpr int kPackMask = EPT == 1 ? 0 : EPT == 2 ? 1 : EPT == 4 ? 3 : EPT == 8 
 template <int EPT, bool PACKED>
 __device__ __forceinline__ bool take_largest(const GateArgs& a, int (&v)[EPT], int lane, float k0, int& mine) {
   constexpr int M = kPackMask<EPT>;
-  bool sure = true;
   if constexpr (PACKED) {
 #pragma unroll
     for (int i = 0; i < EPT; ++i) v[i] = v[i] == kNone ? INT_MIN : (v[i] & ~M) | (M - i);
@@ -257,8 +256,8 @@ __device__ __forceinline__ bool take_largest(const GateArgs& a, int (&v)[EPT], i
     }
   }
   constexpr int kLow = PACKED ? INT_MIN : kNone;
-  float before = 0.f;
   int best = kLow, key = kLow, lane_of = 0;   // lane k: the k-th key and its lane
+  int top = kLow;
   if constexpr (PACKED && EPT <= 8) {
     best = v[0];
   } else {
@@ -271,15 +270,8 @@ __device__ __forceinline__ bool take_largest(const GateArgs& a, int (&v)[EPT], i
   for (int k = 0; k < rounds; ++k) {
     // without the places, which order equal values within a lane only
     const int value = PACKED ? best & ~M : best;
-    const int top = __reduce_max_sync(kAll, value);
+    top = __reduce_max_sync(kAll, value);
     if (top == kLow) break;
-    if (k0 > 0.f) {
-      const float x = of_key(top);
-      // the scores' errors, the bias's roundings and the low bits that packing took
-      if (k > 0 && !(before - x > 2.f * k0 + (fabsf(before) + fabsf(x)) * (PACKED ? (M + 2) * 0x1p-23f : 0x1p-23f))) sure = false;
-      before = x;
-    }
-    if (k == a.K) break;
     const int from = __ffs(__ballot_sync(kAll, value == top)) - 1;  // ids grow with the lane
     const int won = PACKED ? __shfl_sync(kAll, best, from) : top;
     if (lane == k) {
@@ -319,8 +311,18 @@ __device__ __forceinline__ bool take_largest(const GateArgs& a, int (&v)[EPT], i
       if (lane == k) at = p;
     }
   }
-  mine = key == kLow ? -1 : lane_of * EPT + (PACKED ? M - (key & M) : at);
-  return sure;
+  mine = key == kLow || lane >= a.K ? -1 : lane_of * EPT + (PACKED ? M - (key & M) : at);
+  if (k0 > 0.f) {
+    // each of the K against the next one (the last against the first left out): the scores' errors, the
+    // bias's roundings and the low bits that packing took
+    int next = __shfl_down_sync(kAll, key, 1);
+    if (lane == a.K - 1) next = top;
+    const float x = of_key(PACKED ? key & ~M : key), y = of_key(PACKED ? next & ~M : next);
+    const bool near = lane < a.K && key != kLow && next != kLow &&
+                      !(x - y > 2.f * k0 + (fabsf(x) + fabsf(y)) * (PACKED ? (M + 2) * 0x1p-23f : 0x1p-23f));
+    return !__any_sync(kAll, near);
+  }
+  return true;
 }
 
 // The same selection with scores in fp64, for the rows that need it: one value of shared memory an
@@ -386,7 +388,7 @@ __device__ __noinline__ int select_f64(const GateArgs& a, const float* l, int ep
 }
 
 template <typename T, int EPT, bool VEC>
-__global__ void __launch_bounds__(kGateWarps * 32) gate_kernel(GateArgs a) {
+__global__ void __launch_bounds__(kGateWarps * 32, EPT <= 8 ? 12 : 1) gate_kernel(GateArgs a) {
   extern __shared__ double gate_smem[];
   const int lane = lane_id(), warp = warp_id();
   const int t = blockIdx.x * kGateWarps + warp;

@@ -318,6 +318,50 @@ def test_block_streams_graphs_and_concurrent_calls():
     assert torch.equal(held[0], ref) and torch.equal(held[1], ref)
 
 
+@pytest.mark.gpu
+@needs_cuda
+def test_block_slabs_on_streams_and_in_graphs():
+    # slabs launch both kernels: side by side on three streams, and from two captured graphs
+    g = torch.Generator().manual_seed(12)
+    counts = torch.tensor([3, 0, 70, 128, 200, 31], dtype=torch.int32)
+    q, sc = (t.cuda() for t in _rows((6, 200), 1024, g))
+    B, sb = (t.cuda() for t in _weight(6, 512, 1024, g))
+    cnt = counts.cuda()
+
+    def call():
+        out = torch.full((6, 200, 512), 7.0, dtype=torch.bfloat16, device='cuda')
+        return grouped_gemm_fp8_block(q, sc, B, sb, counts=cnt, out=out)
+
+    ref = call()
+    for e, n in enumerate(counts.tolist()):
+        assert (ref[e, n:] == 7).all()
+        if n:
+            _check(ref[e, :n], *_expected(q.cpu(), sc.cpu(), B.cpu(), sb.cpu(), (e, slice(0, n)), e, False), 1024)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for i in range(9):
+        with torch.cuda.stream(streams[i % 3]):
+            outs.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref) for o in outs)
+    graphs, held = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(call())
+        graphs.append(graph)
+    cnt.copy_(counts.flip(0))
+    for graph, s in zip(graphs, streams):
+        with torch.cuda.stream(s):
+            graph.replay()
+    torch.cuda.synchronize()
+    want = call()
+    assert torch.equal(held[0], want) and torch.equal(held[1], want)
+    cnt.zero_()
+    assert (call() == 7).all()
+
+
 def _refusals(dev):
     u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8, device=dev).view(F8)  # noqa: E731
     f = lambda *s: torch.zeros(*s, device=dev)  # noqa: E731
