@@ -24,9 +24,13 @@
 // Two kernels, for groups with many and with few rows:
 //  * many: 128 rows x 256 columns, rows of A on the TMEM lanes; a CTA takes whole tiles. Bound by the
 //    operands' way into shared memory (48 KB a block at 64 bytes a cycle: 768 cycles).
+//    32 groups of 1024 rows, N 4096, K 7168, SwiGLU and pre-activation: 1180 us, 1630 TFLOP/s (1473 us
+//    with MMAs behind `lane == 0` and scales loaded by the threads that use them).
 //  * few (at most kFewTile rows): 256 columns x up to 48 rows, columns of C on the lanes, so that
-//    nothing is spent on rows that are not there. Bound by reading B. Tiles that do not fill a round of the SMs are taken by clusters that divide
-//    K and add their parts through distributed shared memory in a fixed order.
+//    nothing is spent on rows that are not there. Bound by reading B: 32 slabs of 32 rows, the same N
+//    and K: 165 us, 5.8 TB/s (prefetching B into L2 ahead of the copies: 232 us). Tiles that do not fill
+//    a round of the SMs are taken by clusters that divide K and add their parts through distributed
+//    shared memory in a fixed order (one row, N 2048, K 7168: 10.5 us, 13.7 in the other form).
 // Segments take one of the two, by the rows that there are. For slabs, whose counts only the device
 // knows, both are launched where the second is worth it, and each takes its groups.
 //
@@ -62,7 +66,6 @@ constexpr int kFewTile = 48;                     // rows of a tile with few rows
 constexpr int kFewStages = 4, kFewBufs = 4;
 constexpr int kFewCols = 64;                     // TMEM columns of a buffer's half
 constexpr int kFewStageBytes = kBBytes + kFewTile * kBK;
-constexpr int kFewPair = 2;                      // K blocks that are loaded together
 constexpr int kMaxSplit = 8;                     // CTAs of a cluster that divide K
 static_assert(kStages % 2 == 0, "two MMA warps take turns: each must see every phase of its stages' barriers");
 static_assert(kFewTile <= kFewCols && kFewBufs * 2 * kFewCols <= 2 * kBN, "TMEM columns");
@@ -73,7 +76,7 @@ enum BlkEpilogue : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiGLU = 2 };
 // Estimated cycles, from measurements. A K block of a tile takes 900, or 1540 where all SMs read a part of
 // B of their own from memory. A tile with few rows costs 2300 more, and 6000 where a cluster divides K.
 // (Decoding, 32 groups of 32 rows: N 4096, K 7168, 512 tiles: 181 us as many rows, in 4 rounds, 165 as
-// few; N 7168, K 2048, 896 tiles: 91 and 100 us. One row, N 2048, K 7168: 14 and 10.7 us.)
+// few; N 7168, K 2048, 896 tiles: 88 and 98 us. One row, N 2048, K 7168: 13.7 and 10.5 us.)
 __host__ __device__ inline int64_t block_cycles(int64_t ctas, int64_t sms, bool own) { return own && ctas * 2 > sms ? 1540 : 900; }
 __host__ __device__ inline int64_t many_cycles(int64_t tiles, int64_t KB, int64_t sms, bool own) {
   return (tiles + sms - 1) / sms * KB * block_cycles(tiles, sms, own) + 4000;
@@ -706,32 +709,22 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       const BlkTile tl = f.tl;
       const int row = static_cast<int>(f.sp.base) + tl.m0;
       const int slab = a.offsets != nullptr ? 0 : tl.g;
-      // Two blocks at a time, 64 rows of one and of the other in turn: 256 contiguous bytes of each row of
-      // B are asked for together (see kFewPair).
-      for (int kb = f.k0; kb < f.k1; kb += kFewPair) {
-        const int n = min(kFewPair, f.k1 - kb);
-        bool ok = true;
-        for (int p = 0; p < n && ok; ++p)
-          ok = wait_blk(&fempty[(it + p) % kFewStages], (((it + p) / kFewStages) & 1u) ^ 1u, a, &s_abort);
-        if (!ok) break;
+      for (int kb = f.k0; kb < f.k1; ++kb, ++it) {
+        const int s = it % kFewStages;
+        if (!wait_blk(&fempty[s], ((it / kFewStages) & 1u) ^ 1u, a, &s_abort)) break;
         if (elect_one()) {
-          for (int p = 0; p < n; ++p) {
-            const int s = (it + p) % kFewStages;
-            mbar_arrive_expect_tx(&ffull[s], kFewStageBytes);
-            tma_load_3d(smem + s * kFewStageBytes + kBBytes, &tmA, &ffull[s], (kb + p) * kBK, row, slab);
-          }
+          mbar_arrive_expect_tx(&ffull[s], kFewStageBytes);
+          uint8_t* db = smem + s * kFewStageBytes;
+          if (B_MN) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            for (int p = 0; p < n; ++p) {
-              const int s = (it + p) % kFewStages;
-              uint8_t* db = smem + s * kFewStageBytes + j * (64 * kBK);
-              if (B_MN) tma_load_3d(db, &tmB, &ffull[s], tl.n0 + (j >> 1) * 128, (kb + p) * kBK + (j & 1) * 64, tl.g);
-              else tma_load_3d(db, &tmB, &ffull[s], (kb + p) * kBK, tl.n0 + j * 64, tl.g);
-            }
+            for (int j = 0; j < kBN / 128; ++j)
+              tma_load_3d(db + j * (128 * kBK), &tmB, &ffull[s], tl.n0 + 128 * j, kb * kBK, tl.g);
+          } else {
+            tma_load_3d(db, &tmB, &ffull[s], kb * kBK, tl.n0, tl.g);
           }
+          tma_load_3d(db + kBBytes, &tmA, &ffull[s], kb * kBK, row, slab);
         }
         __syncwarp();
-        it += n;
       }
     }
     if (s_abort) {  // copies in flight land before the CTA's shared memory is given up
@@ -1016,8 +1009,7 @@ int few_launch(const CUtensorMap& ma, const CUtensorMap& mb, const BlkArgs& a, i
 // One call: the forms that its rows take, and the launches. `rows_known`: the rows of all groups together
 // (an upper bound), or 0 where only the device knows (slabs).
 template <int EPI, bool B_MN>
-void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMap& mb, const CUtensorMap& mbf,
-                  BlkArgs a, int64_t rows_known,
+void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMap& mb, BlkArgs a, int64_t rows_known,
                   cudaStream_t stream) {
   const int64_t ntn = (a.N + kBN - 1) / kBN, KB = (a.K + kBK - 1) / kBK;
   // tiles of groups with few rows: one a group (slabs), or as many as the rows make
@@ -1043,7 +1035,7 @@ void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMa
     // a decoding step, a tile a group, decides whether the form for few rows is worth its launch
     a.form = least >= many_cycles(few, KB, a.sms, true) ? kAllMany : a.rows <= kFewTile ? kAllFew : kBothForms;
   }
-  if (a.form != kAllMany) few_launch<EPI, B_MN>(mf, mbf, a, a.few_grid, a.split, stream);
+  if (a.form != kAllMany) few_launch<EPI, B_MN>(mf, mb, a, a.few_grid, a.split, stream);
   if (a.form == kAllFew) return;
   constexpr int smem = 1024 + kStages * kStageBytes + kEpiWarps * kWarpStage;
   auto kfn = gemm_block_kernel<EPI, B_MN>;
@@ -1168,17 +1160,15 @@ void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at:
                                 : map_u8_3d(A.data_ptr(), K, a.rows, 1, s1, s1 * a.rows, kFewTile);
   const CUtensorMap mb = b_kn ? map_u8_3d(B.data_ptr(), N, K, a.G, N, N * K, kBK)
                               : map_u8_3d(B.data_ptr(), K, N, a.G, K, N * K, kBN);
-  const CUtensorMap mbf = b_kn ? map_u8_3d(B.data_ptr(), N, K, a.G, N, N * K, 64)
-                               : map_u8_3d(B.data_ptr(), K, N, a.G, K, N * K, 64);
   const int all = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   a.sms = num_sms > 0 ? static_cast<int>(std::min<int64_t>(num_sms, all)) : all;
   const int64_t known = masked ? 0 : a.rows;
   auto stream = at::cuda::getCurrentCUDAStream();
-  if (epilogue == kOutSwiGLU) launch_block<kOutSwiGLU, false>(ma, mf, mb, mbf, a, known, stream);
-  else if (epilogue == kOutBF16 && b_kn) launch_block<kOutBF16, true>(ma, mf, mb, mbf, a, known, stream);
-  else if (epilogue == kOutBF16) launch_block<kOutBF16, false>(ma, mf, mb, mbf, a, known, stream);
-  else if (b_kn) launch_block<kOutF32, true>(ma, mf, mb, mbf, a, known, stream);
-  else launch_block<kOutF32, false>(ma, mf, mb, mbf, a, known, stream);
+  if (epilogue == kOutSwiGLU) launch_block<kOutSwiGLU, false>(ma, mf, mb, a, known, stream);
+  else if (epilogue == kOutBF16 && b_kn) launch_block<kOutBF16, true>(ma, mf, mb, a, known, stream);
+  else if (epilogue == kOutBF16) launch_block<kOutBF16, false>(ma, mf, mb, a, known, stream);
+  else if (b_kn) launch_block<kOutF32, true>(ma, mf, mb, a, known, stream);
+  else launch_block<kOutF32, false>(ma, mf, mb, a, known, stream);
 }
 
 }  // namespace b200ep
