@@ -19,8 +19,8 @@
 // one token, its experts in the lanes' registers (16-byte loads and stores where the rows allow).
 // Values are compared as integers of the same order, so that one redux finds the warp's largest.
 // Bound by instruction issue (about 1000 a row of 256 experts, 8 groups, 8 chosen): 16384 such tokens
-// forward and backward in 38 us where their bytes would take 6 (59 us with values compared as floats by
-// shuffles, 4-byte accesses and ids looked for in every lane); one token 3.9 us (7.2 before), of which
+// forward and backward in 37 us where their bytes would take 6 (59 us with values compared as floats by
+// shuffles, 4-byte accesses and ids looked for in every lane); one token 3.7 us (7.2 before), of which
 // 2.5 are a launch.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -244,15 +244,21 @@ __device__ __forceinline__ bool take_largest(const GateArgs& a, int (&v)[EPT], i
   if constexpr (PACKED) {
 #pragma unroll
     for (int i = 0; i < EPT; ++i) v[i] = v[i] == kNone ? INT_MIN : (v[i] & ~M) | (M - i);
-    if constexpr (EPT <= 8) {   // each lane's keys in descending order: bubbles of compare and exchange
-#pragma unroll
-      for (int i = EPT - 1; i > 0; --i)
-#pragma unroll
-        for (int j = 0; j < i; ++j) {
-          const int hi = max(v[j], v[j + 1]), lo = min(v[j], v[j + 1]);
-          v[j] = hi;
-          v[j + 1] = lo;
-        }
+    if constexpr (EPT <= 8) {   // each lane's keys in descending order, by a sorting network of 1, 5 or 19 exchanges
+      auto order = [&](int i, int j) {
+        const int hi = max(v[i], v[j]), lo = min(v[i], v[j]);
+        v[i] = hi;
+        v[j] = lo;
+      };
+      if constexpr (EPT == 8) {
+        order(0, 2), order(1, 3), order(4, 6), order(5, 7), order(0, 4), order(1, 5), order(2, 6), order(3, 7);
+        order(0, 1), order(2, 3), order(4, 5), order(6, 7), order(2, 4), order(3, 5), order(1, 4), order(3, 6);
+        order(1, 2), order(3, 4), order(5, 6);
+      } else if constexpr (EPT == 4) {
+        order(0, 2), order(1, 3), order(0, 1), order(2, 3), order(1, 2);
+      } else if constexpr (EPT == 2) {
+        order(0, 1);
+      }
     }
   }
   constexpr int kLow = PACKED ? INT_MIN : kNone;
@@ -279,9 +285,10 @@ __device__ __forceinline__ bool take_largest(const GateArgs& a, int (&v)[EPT], i
       lane_of = from;
     }
     if constexpr (PACKED && EPT <= 8) {
-      const bool mine_goes = lane == from;
+      if (lane == from) {
 #pragma unroll
-      for (int i = 0; i < EPT; ++i) v[i] = mine_goes ? (i + 1 < EPT ? v[i + 1] : INT_MIN) : v[i];
+        for (int i = 0; i < EPT; ++i) v[i] = i + 1 < EPT ? v[i + 1] : INT_MIN;
+      }
       best = v[0];
     } else if constexpr (PACKED) {
       if (lane == from) {
