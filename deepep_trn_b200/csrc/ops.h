@@ -155,6 +155,7 @@ void transpose(const at::Tensor& in, at::Tensor out);
 // quant.cu
 void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_scale);
 void dequant_fp8(const at::Tensor& q, const at::Tensor& scales, at::Tensor out);
-std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w);
+std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w, const OptTensor& q_out,
+                                                    const OptTensor& scales_out);
 
 }  // namespace b200ep

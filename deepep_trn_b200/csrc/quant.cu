@@ -178,26 +178,44 @@ __global__ void __launch_bounds__(kWqThreads, sizeof(T) == 2 && VEC ? 3 : 2)
   }
 }
 
-std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w) {
+std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w, const OptTensor& q_out,
+                                                    const OptTensor& scales_out) {
   TORCH_CHECK((w.dim() == 2 || w.dim() == 3) && unit_inner(w), "w must be [N, K] or [G, N, K] with unit inner stride");
   TORCH_CHECK(w.scalar_type() == at::kFloat || w.scalar_type() == at::kBFloat16 || w.scalar_type() == at::kHalf,
               "w must be fp32, bf16 or fp16");
-  if (!w.is_cuda()) return {};  // CPU tensors: the checks alone
-  const c10::cuda::CUDAGuard guard(w.device());
   const int64_t G = w.dim() == 3 ? w.size(0) : 1, N = w.size(-2), K = w.size(-1);
   TORCH_CHECK(N < (1 << 30) && K < (1 << 30), "sizes below 2^30");
   const int64_t NB = (N + 127) / 128, KB = (K + 127) / 128;
-  auto shape = w.sizes().vec();
-  at::Tensor q = at::detail::empty_cuda(shape, at::kFloat8_e4m3fn, w.device(), c10::nullopt);
-  shape[shape.size() - 2] = NB;
-  shape.back() = KB;
-  at::Tensor sc = at::detail::empty_cuda(shape, at::kFloat, w.device(), c10::nullopt);
+  auto shape = w.sizes().vec(), scales_shape = shape;
+  scales_shape[shape.size() - 2] = NB;
+  scales_shape.back() = KB;
+  TORCH_CHECK(q_out.has_value() == scales_out.has_value(), "an output is a pair");
+  if (q_out.has_value()) {
+    TORCH_CHECK(q_out->device() == w.device() && q_out->scalar_type() == at::kFloat8_e4m3fn && q_out->sizes() == shape &&
+                    q_out->is_contiguous(),
+                "the output must be contiguous e4m3 of w's sizes on its device");
+    TORCH_CHECK(scales_out->device() == w.device() && scales_out->scalar_type() == at::kFloat &&
+                    scales_out->sizes() == scales_shape && scales_out->is_contiguous(),
+                "the output's scales must be contiguous fp32, one a 128 x 128 block, on w's device");
+  }
+  if (!w.is_cuda()) return {};  // CPU tensors: the checks alone
+  const c10::cuda::CUDAGuard guard(w.device());
+  at::Tensor q, sc;
+  if (q_out.has_value()) {
+    q = *q_out;
+    sc = *scales_out;
+  } else {
+    q = at::detail::empty_cuda(shape, at::kFloat8_e4m3fn, w.device(), c10::nullopt);
+    sc = at::detail::empty_cuda(scales_shape, at::kFloat, w.device(), c10::nullopt);
+  }
+  // 8 values of a row are stored at once: an output of odd offset is written element by element
+  const bool aligned = (reinterpret_cast<uintptr_t>(q.data_ptr()) & 7) == 0;
   const int64_t blocks = G * NB * KB;
   if (blocks == 0) return {q, sc};
   TORCH_CHECK(blocks < (1ll << 31), "too many blocks");
   const int64_t es = w.element_size(), row = w.stride(-2), group = w.dim() == 3 ? w.stride(0) : 0;
-  const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0 && row * es % 16 == 0 &&
-                   group * es % 16 == 0;
+  const bool vec = aligned && K % 8 == 0 && (reinterpret_cast<uintptr_t>(w.data_ptr()) & 15) == 0 &&
+                   row * es % 16 == 0 && group * es % 16 == 0;
   auto s = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto zero) {
     using T = decltype(zero);

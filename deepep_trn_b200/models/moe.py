@@ -215,7 +215,8 @@ class MoELayer(nn.Module):
         self.gate = dict(gate) if gate is not None else None
         # e4m3 dispatch and experts with fp32 block scales, in training too
         self.fp8_block = fp8_block
-        self._fp8_cache = None
+        self._fp8_cache = None    # fp8_experts
+        self._block_copy = self._block_key = None   # fp8_block: what quantize_weights made, and of which weights
         self.hidden, self.intermediate = hidden, intermediate
         self.num_experts, self.topk = num_experts, topk
         EL = num_experts // R
@@ -254,25 +255,48 @@ class MoELayer(nn.Module):
                 self._fp8_cache = (key, q1, G.fp8_scale_tiles(s1, EL), q2, G.fp8_scale_tiles(s2, EL))
         return self._fp8_cache[1:]
 
+    def _weights_key(self):
+        """What a write to the weights usually changes (not one through ``w.data``)."""
+        return tuple((w.device, w.data_ptr(), 0 if w.is_inference() else w._version) for w in (self.w1, self.w2))
+
+    @torch.no_grad()
+    def quantize_weights(self) -> None:
+        """Quantises the expert weights of an ``fp8_block`` layer into a copy that ``forward_low_latency`` and
+        calls without gradients then read instead of quantising the weights themselves (0.47 ms for 32
+        experts of 4096 x 7168). Call it again after a change of the weights: it writes into the same storage, so
+        the replays of a captured step see the new weights from then on. Calls on other streams are ordered
+        behind it as behind any write to the weights. The copy is left aside once the weights' version or
+        address differs, and after a call with gradients, which an update follows; only a write through
+        ``w.data`` outside of training goes unseen."""
+        if not self.fp8_block:
+            raise ValueError('quantize_weights needs fp8_block=True')
+        if self.w1.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('quantize_weights must be called outside of a capture')
+        kept = self._block_copy
+        if kept is not None and not all(q.shape == w.shape and q.device == w.device
+                                        for q, w in ((kept[0], self.w1), (kept[2], self.w2))):
+            kept = None
+        self._block_key = None
+        self._block_copy = (*G.quantize_fp8_weight(self.w1, out=kept and kept[:2]),
+                            *G.quantize_fp8_weight(self.w2, out=kept and kept[2:]))
+        self._block_key = self._weights_key()
+
     def _block_weights(self, train: bool):
-        """(q1, s1, q2, s2): e4m3 expert weights with 128x128 fp32 scales. In training every call quantises
-        them (0.47 ms for 32 experts of 4096 x 7168): an optimizer that writes through ``w.data`` changes
-        neither version nor address, so no kept copy could be told from an old one. Without gradients a copy
-        is kept, until version or address change or the next call with gradients."""
-        key = None if train else (self.w1._version, self.w2._version, self.w1.data_ptr(), self.w2.data_ptr())
-        if train or self._fp8_cache is None or self._fp8_cache[0] != key:
-            with torch.no_grad():
-                wq = (*G.quantize_fp8_weight(self.w1), *G.quantize_fp8_weight(self.w2))
-            if train:
-                return wq
-            self._fp8_cache = (key, *wq)
-        return self._fp8_cache[1:]
+        """(q1, s1, q2, s2): e4m3 expert weights with 128x128 fp32 scales, quantised in this call, or without
+        gradients the copy of ``quantize_weights``. (An optimizer that writes through ``w.data`` changes neither
+        version nor address: in training no kept copy could be told from an old one.)"""
+        if not train and self._block_key is not None and self._block_key == self._weights_key():
+            return self._block_copy
+        with torch.no_grad():
+            return (*G.quantize_fp8_weight(self.w1), *G.quantize_fp8_weight(self.w2))
 
     @torch.no_grad()
     def forward_low_latency(self, x: torch.Tensor, num_max_tokens_per_rank: int) -> torch.Tensor:
         """A generation step (``fp8_block`` layers): low-latency dispatch -> expert slabs -> combine. ``x`` holds
         at most ``num_max_tokens_per_rank`` tokens, which all ranks give alike. Nothing waits on the host, so
-        the step can be captured into a CUDA graph after one call."""
+        the step can be captured into a CUDA graph after one call. Captured after ``quantize_weights`` it reads
+        that copy, which the next ``quantize_weights`` renews in place; captured without, every replay quantises
+        the weights as they are then."""
         if not self.fp8_block:
             raise ValueError('forward_low_latency needs fp8_block=True')
         q1, s1, q2, s2 = self._block_weights(train=False)
@@ -311,8 +335,9 @@ class MoELayer(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         train = torch.is_grad_enabled()
-        if train:
-            self._fp8_cache = None   # the weights are about to change, perhaps without a trace (see _block_weights)
+        if train and (self.w1.requires_grad or self.w2.requires_grad):
+            # the weights are about to change, perhaps without a trace (see _block_weights)
+            self._fp8_cache = self._block_key = None
         if self.fp8_experts and not train:
             return self._forward_fp8(x)
         if self.fp8_block:

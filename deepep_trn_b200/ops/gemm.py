@@ -123,16 +123,24 @@ def grouped_gemm_fp8(A, sa, B, sb, offsets, out=None, epilogue: str = 'bf16', h_
 FP8_BLOCK_EPILOGUES = {'bf16': 0, 'f32': 1, 'swiglu': 2}
 
 
-def quantize_fp8_weight(w: torch.Tensor):
+def quantize_fp8_weight(w: torch.Tensor, out=None):
     """e4m3 copy of ``w`` [N, K] or [G, N, K] (fp32, bf16 or fp16) with one fp32 scale per
     128 x 128 block (the last blocks of a side may be short): ``(q, scales [.., ceil(N/128),
     ceil(K/128)])`` with ``w ~= q * scale``, ``scale = max(amax, 1e-4) / 448``. The operand format
-    of ``grouped_gemm_fp8_block``; a transposed product reads the same pair (``b_layout='kn'``)."""
-    if not w.is_cuda:
-        if available():
-            load().quant_fp8_weight(w)   # the argument checks
-        return quantize_fp8_128x128(w)
-    return load().quant_fp8_weight(w)
+    of ``grouped_gemm_fp8_block``; a transposed product reads the same pair (``b_layout='kn'``).
+    ``out``: a contiguous pair ``(q, scales)`` to write, which is returned."""
+    q, sc = out if out is not None else (None, None)
+    if w.is_cuda:
+        res = load().quant_fp8_weight(w, q, sc)
+        return out if out is not None else res
+    if available():
+        load().quant_fp8_weight(w, q, sc)   # the argument checks
+    res = quantize_fp8_128x128(w)
+    if out is None:
+        return res
+    q.view(torch.uint8).copy_(res[0].view(torch.uint8))
+    sc.copy_(res[1])
+    return out
 
 
 def grouped_gemm_fp8_block(A, sa, B, sb, offsets=None, counts=None, out=None, epilogue: str = 'bf16',
