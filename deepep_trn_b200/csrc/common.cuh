@@ -334,18 +334,22 @@ __device__ __forceinline__ float pow2_ceil(float s) {
 // One lane's share of a 1x128 block quantisation: 8 contiguous values, the
 // other 15 lanes of the same half-warp hold the rest of the block. Every lane of
 // the warp must call this (it shuffles); inactive lanes pass zeros.
-// scale = max(amax, 1e-4) / 448 (or its power-of-two ceiling); q = rn_satfinite(v * (448 / amax)).
+// scale = max(amax, amax_floor) / 448 (or its power-of-two ceiling); q = rn_satfinite(v * (448 / amax)). The floor
+// of activations and weights is 1e-4, that of gradients, which have no natural size, near the smallest normal number
+// (the caller gives it).
+constexpr float kAmaxFloor = 1e-4f;
 struct Quant8 {
   uint2 q;
   float scale;
 };
-__device__ __forceinline__ Quant8 quant8_e4m3(const float (&v)[8], bool round_scale) {
+__device__ __forceinline__ Quant8 quant8_e4m3(const float (&v)[8], bool round_scale,
+                                                float amax_floor = kAmaxFloor) {
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
 #pragma unroll
   for (int m = 8; m >= 1; m >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
-  amax = fmaxf(amax, 1e-4f);
+  amax = fmaxf(amax, amax_floor);
   float scale, inv;
   if (round_scale) {
     scale = pow2_ceil(__fdiv_rn(amax, 448.f));
@@ -379,7 +383,8 @@ __device__ __forceinline__ void load8(float (&v)[8], const T16* p, bool act) {
 // Four 256-element chunks are loaded before any is quantised (four loads in flight per lane).
 template <typename T16>
 __device__ __forceinline__ void warp_quant_row(uint8_t* __restrict__ dst, float* __restrict__ scales,
-                                               const T16* __restrict__ src, int H, bool round_scale) {
+                                               const T16* __restrict__ src, int H, bool round_scale,
+                                               float amax_floor = kAmaxFloor) {
   const int lane = lane_id();
   for (int c0 = 0; c0 < H; c0 += 1024) {
     float v[4][8];
@@ -391,7 +396,7 @@ __device__ __forceinline__ void warp_quant_row(uint8_t* __restrict__ dst, float*
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int off = c0 + u * 256 + lane * 8;
-      const Quant8 r = quant8_e4m3(v[u], round_scale);
+      const Quant8 r = quant8_e4m3(v[u], round_scale, amax_floor);
       if (off < H) {
         *reinterpret_cast<uint2*>(dst + off) = r.q;
         if ((lane & 15) == 0) scales[off / 128] = r.scale;

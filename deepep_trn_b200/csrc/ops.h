@@ -153,7 +153,7 @@ void swiglu_bwd(const at::Tensor& dh, const at::Tensor& pre, at::Tensor dpre);
 void transpose(const at::Tensor& in, at::Tensor out);
 
 // quant.cu
-void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_scale);
+void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_scale, double amax_floor);
 void dequant_fp8(const at::Tensor& q, const at::Tensor& scales, at::Tensor out);
 std::tuple<at::Tensor, at::Tensor> quant_fp8_weight(const at::Tensor& w, const OptTensor& q_out,
                                                     const OptTensor& scales_out);

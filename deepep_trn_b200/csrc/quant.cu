@@ -11,14 +11,14 @@ namespace b200ep {
 template <typename T16>
 __global__ void __launch_bounds__(256) quant_fp8_kernel(const T16* __restrict__ x, uint8_t* __restrict__ q,
                                                         float* __restrict__ scales, int64_t T, int H,
-                                                        int round_scale) {
+                                                        int round_scale, float amax_floor) {
   const int64_t gw = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int64_t GW = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
   for (int64_t t = gw; t < T; t += GW)
-    warp_quant_row<T16>(q + t * H, scales + t * (H / 128), x + t * H, H, round_scale);
+    warp_quant_row<T16>(q + t * H, scales + t * (H / 128), x + t * H, H, round_scale, amax_floor);
 }
 
-void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_scale) {
+void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_scale, double amax_floor) {
   const c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(x.is_contiguous() && q.is_contiguous() && scales.is_contiguous(), "contiguous tensors expected");
   const int H = static_cast<int>(x.size(-1));
@@ -26,17 +26,19 @@ void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_
   const int64_t T = x.numel() / H;
   TORCH_CHECK(q.element_size() == 1 && q.numel() == x.numel(), "q must be a 1-byte tensor shaped like x");
   TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.numel() == T * (H / 128), "scales must be fp32 [.., H/128]");
+  // below, the scale would be subnormal or 448 / amax infinite
+  TORCH_CHECK(amax_floor >= 0x1p-116 && amax_floor <= 448., "the floor of amax must be between 2^-116 and 448");
   if (T == 0) return;
   const int blocks = static_cast<int>(std::min<int64_t>((T + 7) / 8, 148 * 16));
   auto stream = at::cuda::getCurrentCUDAStream();
   if (x.scalar_type() == at::kHalf)
     quant_fp8_kernel<__half><<<blocks, 256, 0, stream>>>(reinterpret_cast<const __half*>(x.data_ptr()),
                                                         static_cast<uint8_t*>(q.data_ptr()), scales.data_ptr<float>(),
-                                                        T, H, round_scale);
+                                                        T, H, round_scale, static_cast<float>(amax_floor));
   else
     quant_fp8_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(
         reinterpret_cast<const __nv_bfloat16*>(x.data_ptr()), static_cast<uint8_t*>(q.data_ptr()),
-        scales.data_ptr<float>(), T, H, round_scale);
+        scales.data_ptr<float>(), T, H, round_scale, static_cast<float>(amax_floor));
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

@@ -31,11 +31,15 @@ import torch.nn as nn
 
 from ..ops import gemm as G
 from ..ops import moe_ops as MO
-from ..ops.quant import dequantize_fp8, quantize_fp8
+from ..ops.quant import GRAD_AMAX_FLOOR, dequantize_fp8, quantize_fp8
 from ..utils.profiling import timer
 
 
 _OFFS: dict = {}
+
+
+def _quantize_grad(d):
+    return quantize_fp8(d, amax_floor=GRAD_AMAX_FLOOR)
 
 
 def _single_segment(T: int, device) -> torch.Tensor:
@@ -177,9 +181,9 @@ class _MoEBlockFunction(torch.autograd.Function):
         with timer.stage('moe.bwd.unpermute'):
             d_o, d_recv_w = MO.unpermute_bwd(dy_recv, o, pos, recv_w, offsets, counts)
         with timer.stage('moe.bwd.dgrad'):
-            dh = G.grouped_gemm_fp8_block(*quantize_fp8(d_o), q2, s2, offsets, b_layout='kn')        # d_o @ W2[e]
+            dh = G.grouped_gemm_fp8_block(*_quantize_grad(d_o), q2, s2, offsets, b_layout='kn')        # d_o @ W2[e]
             dpre = MO.swiglu_bwd(dh, pre)
-            drows = G.grouped_gemm_fp8_block(*quantize_fp8(dpre), q1, s1, offsets, b_layout='kn')    # dpre @ W1[e]
+            drows = G.grouped_gemm_fp8_block(*_quantize_grad(dpre), q1, s1, offsets, b_layout='kn')    # dpre @ W1[e]
         with timer.stage('moe.bwd.wgrad'):
             dW2 = G.grouped_gemm_wgrad(d_o, dequantize_fp8(h, hs), offsets, out_dtype=ctx.w_dtypes[1])
             dW1 = G.grouped_gemm_wgrad(dpre, dequantize_fp8(rq, rs), offsets, out_dtype=ctx.w_dtypes[0])

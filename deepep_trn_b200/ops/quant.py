@@ -4,18 +4,25 @@ from __future__ import annotations
 
 import torch
 
-from ..utils.codec import dequantize_fp8_1x128, quantize_fp8_1x128
+from ..utils.codec import FP8_AMAX_FLOOR, dequantize_fp8_1x128, quantize_fp8_1x128
 from ._ext import load
 
 
-def quantize_fp8(x: torch.Tensor, round_scale: bool = False):
+# Gradients have no natural size (a mean over a large batch puts them at 1e-8 or below), so that the floor of
+# activations would take them for zeros: 2^-116 keeps amax / 448 normal and 448 / amax finite in fp32.
+GRAD_AMAX_FLOOR = 2.0 ** -116
+
+
+def quantize_fp8(x: torch.Tensor, round_scale: bool = False, amax_floor: float = FP8_AMAX_FLOOR):
+    """e4m3 with one fp32 scale ``max(amax, amax_floor) / 448`` per 128 channels (``round_scale``: its power-of-two
+    ceiling). Blocks far below the floor lose their values; gradients take ``GRAD_AMAX_FLOOR``."""
     if not x.is_cuda:
-        return quantize_fp8_1x128(x, round_scale)
+        return quantize_fp8_1x128(x, round_scale, amax_floor)
     x = x.contiguous()
     H = x.shape[-1]
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     s = torch.empty(*x.shape[:-1], H // 128, dtype=torch.float32, device=x.device)
-    load().quant_fp8(x, q.view(torch.uint8), s, round_scale)
+    load().quant_fp8(x, q.view(torch.uint8), s, round_scale, amax_floor)
     return q, s
 
 

@@ -88,18 +88,20 @@ def _pow2_ceil(s: torch.Tensor) -> torch.Tensor:
     return (exp << 23).view(torch.float32)
 
 
-def quantize_fp8_1x128(x: torch.Tensor, round_scale: bool = False):
+def quantize_fp8_1x128(x: torch.Tensor, round_scale: bool = False, amax_floor: float = FP8_AMAX_FLOOR):
     """Per-token, per-128-channel e4m3 quantisation (torch definition of the kernel).
 
     Returns ``(q [.., H] float8_e4m3fn, scales [.., H/128] fp32)`` with
     ``x ~= q * scale`` per block. With ``round_scale`` the scale is rounded up to
-    a power of two (UE8M0-representable).
+    a power of two (UE8M0-representable). ``amax_floor`` is the least amax of a block.
     """
+    if not 2.0 ** -116 <= amax_floor <= FP8_MAX:
+        raise RuntimeError('the floor of amax must be between 2^-116 and 448')
     H = x.shape[-1]
     if H % FP8_BLOCK:
         raise ValueError(f'hidden={H} must be a multiple of {FP8_BLOCK} for fp8 block scales')
     xf = x.float().reshape(*x.shape[:-1], H // FP8_BLOCK, FP8_BLOCK)
-    amax = xf.abs().amax(-1).clamp_min(FP8_AMAX_FLOOR)
+    amax = xf.abs().amax(-1).clamp_min(amax_floor)
     # IEEE divisions tensor by tensor (a python scalar on the left would become
     # reciprocal-then-multiply in torch and round differently from the kernel)
     c448 = torch.full_like(amax, FP8_MAX)
