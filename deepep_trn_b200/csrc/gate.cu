@@ -148,9 +148,11 @@ __device__ __forceinline__ void store_row(T* __restrict__ row, const float (&l)[
 __device__ __forceinline__ int group_of(const GateArgs& a, int e) { return static_cast<int>((e + 0.5f) * a.inv_gs); }
 
 // The groups' part of the selection: of the warp's keys v (lane holds experts lane * EPT + i) those of
-// the groups that are not kept become kNone. k0 (if not 0) bounds the error of one score; to it come the
-// roundings of the bias's and the groups' sums, two units of 2^-24 of a value. False is returned if some
-// order that matters is not certain.
+// the groups that are not kept become kNone. k0 (if not 0) bounds the error of one score. A group's value is
+// certain to 2 k0 and the roundings of score + bias and of the sum, which go with the summands and not with the
+// sum, in which they may cancel: below 2^-23 (|t0| + |t1|), of which twice is taken for the bounds' own
+// roundings. (The bounds grow with the value, so the two largest are the two largest within them too.) False is
+// returned unless the least that a kept group can be is above the most that any other can be.
 template <int EPT>
 __device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], int* buf, int lane, float k0) {
   int t0 = kNone, t1 = kNone;   // the two largest of the group that this lane helps to scan
@@ -192,9 +194,10 @@ __device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], in
   }
   // the sum counts the second value only where there is one
   const int grp = lane >> shift;
-  int gv = grp >= a.n ? kNone : a.top2 && t1 > kNone ? key_of(of_key(t0) + of_key(t1) + 0.f) : t0;
+  const float x0 = of_key(t0), x1 = a.top2 && t1 > kNone ? of_key(t1) : 0.f;
+  const float x = x0 + x1;
+  int gv = grp >= a.n ? kNone : key_of(x + 0.f);
   bool in = false;
-  int worst_in = INT_MAX;
 #pragma unroll 1
   for (int j = 0; j < a.g; ++j) {   // the best group left; its lanes hold the same value, ties go to the first
     const int top = __reduce_max_sync(kAll, gv);
@@ -204,13 +207,14 @@ __device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], in
       in = true;
       gv = kNone;
     }
-    worst_in = top;
   }
   bool sure = true;
   if (k0 > 0.f) {
-    const int best_out = __reduce_max_sync(kAll, gv);
-    const float x = of_key(worst_in), y = of_key(best_out);
-    sure = best_out == kNone || x - y > 4.f * k0 + (fabsf(x) + fabsf(y)) * 0x1p-22f;
+    // (infinities may make a NaN of a bound: fmaxf and fminf put the infinity there that is not certain)
+    const float e = 2.f * k0 + fabsf(x0) * 0x1p-22f + fabsf(x1) * 0x1p-22f;
+    const int least_in = __reduce_min_sync(kAll, in ? key_of(fmaxf(x - e, -INFINITY)) : INT_MAX);
+    const int most_out = __reduce_max_sync(kAll, gv > kNone ? key_of(fminf(x + e, INFINITY)) : kNone);
+    sure = most_out == kNone || least_in > most_out;
   }
   if (a.reg_lanes > 0) {
 #pragma unroll
