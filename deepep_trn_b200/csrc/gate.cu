@@ -196,7 +196,9 @@ __device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], in
   const int grp = lane >> shift;
   const float x0 = of_key(t0), x1 = a.top2 && t1 > kNone ? of_key(t1) : 0.f;
   const float x = x0 + x1;
-  int gv = grp >= a.n ? kNone : key_of(x + 0.f);
+  // (two values of the type's lowest make -inf of the sum: the group stays available)
+  const float xa = x0 > -INFINITY ? fmaxf(x, -FLT_MAX) : x0;
+  int gv = grp >= a.n ? kNone : key_of(xa + 0.f);
   bool in = false;
 #pragma unroll 1
   for (int j = 0; j < a.g; ++j) {   // the best group left; its lanes hold the same value, ties go to the first
@@ -213,7 +215,7 @@ __device__ __forceinline__ bool keep_groups(const GateArgs& a, int (&v)[EPT], in
     // (infinities may make a NaN of a bound: fmaxf and fminf put the infinity there that is not certain)
     const float e = 2.f * k0 + fabsf(x0) * 0x1p-22f + fabsf(x1) * 0x1p-22f;
     const int least_in = __reduce_min_sync(kAll, in ? key_of(fmaxf(x - e, -INFINITY)) : INT_MAX);
-    const int most_out = __reduce_max_sync(kAll, gv > kNone ? key_of(fminf(x + e, INFINITY)) : kNone);
+    const int most_out = __reduce_max_sync(kAll, gv > kNone ? key_of(fminf(xa + e, INFINITY)) : kNone);
     sure = most_out == kNone || least_in > most_out;
   }
   if (a.reg_lanes > 0) {

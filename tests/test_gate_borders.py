@@ -40,3 +40,32 @@ def test_group_sums_that_cancel_in_wide_rows(E, n, g):
     bias = torch.full((E,), -1e4)
     bias[::E // n] = 1e4
     _same_ids(x, 2, scoring='sigmoid', bias=bias, num_groups=n, topk_groups=g)
+
+
+@needs_cuda
+@pytest.mark.parametrize('scoring', ['sigmoid', 'softmax'])
+@pytest.mark.parametrize('group_score', ['top2', 'max'])
+@pytest.mark.parametrize('E,n', [(16, 4), (256, 8), (160, 8), (6, 3)])
+def test_biases_of_the_lowest_value(scoring, group_score, E, n):
+    # closed by the lowest value an expert comes last, but is available: two of them add up to less than fp32
+    # holds, and their group still comes before one that has nothing left
+    low = torch.finfo(torch.float32).min
+    x = torch.randn(3000, E, generator=torch.Generator().manual_seed(E))
+    gs = E // n
+    bias = torch.zeros(E)
+    bias[gs:2 * gs] = low
+    bias[2 * gs:3 * gs] = -math.inf
+    if n > 3:
+        bias[3 * gs:4 * gs] = low
+    for g, k in ((1, 1), (2, gs + 1), (n, min(32, 2 * gs))):
+        _same_ids(x, min(k, 32, g * gs), scoring=scoring, bias=bias, num_groups=n, topk_groups=g,
+                  group_score=group_score)
+    bias[:gs] = low
+    _same_ids(x, min(gs, 32), scoring=scoring, bias=bias, num_groups=n, topk_groups=2, group_score=group_score)
+    bias = torch.full((E,), low)
+    bias[::gs] = 0.25      # one open expert a group
+    _same_ids(x, 2, scoring=scoring, bias=bias, num_groups=n, topk_groups=2, group_score=group_score)
+    high = torch.finfo(torch.float32).max
+    bias[1::gs] = high
+    bias[::gs] = high
+    _same_ids(x, 2, scoring=scoring, bias=bias, num_groups=n, topk_groups=2, group_score=group_score)
