@@ -137,16 +137,18 @@ template <int BYTES>
 __device__ __forceinline__ void cp_async(void* smem, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(src), "n"(BYTES) : "memory");
 }
-// Bounded wait (the clock and the abort flag are looked at once in 256 polls). Every hand-over between
-// warps through an mbarrier takes about 130 cycles; with a suspend-time hint it took longer still.
+// Bounded wait of a whole warp, whose lanes leave it together with one answer: what follows (elect.sync, TMEM
+// loads, barriers) needs all of them. The clock and the abort flag are looked at once in 256 polls, of which
+// each is suspended for up to 4 us. Every hand-over between warps through an mbarrier takes about 130 cycles;
+// with a suspend-time hint it took longer still.
 __device__ __forceinline__ bool wait_blk(uint64_t* bar, uint32_t parity, const BlkArgs& a, volatile int* abort) {
   uint64_t t0 = 0;
   for (uint32_t n = 1;; ++n) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     if ((n & 255u) == 0u) {
       const uint64_t now = global_ns();
       if (t0 == 0) t0 = now;
-      if (*abort || now - t0 > a.timeout_ns) {
+      if (__any_sync(0xffffffffu, *abort || now - t0 > a.timeout_ns)) {
         atomicExch(a.error, 1u);
         *abort = 1;
         return false;
@@ -392,13 +394,15 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
     if (warp == 0) {
       // ------------------------------------------------------------------ TMA producer
       uint32_t it = 0;
+      bool ok = true;
       BlkTile tl;
-      for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
+      for (int t = blockIdx.x; ok && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
         const int row = static_cast<int>(group_span(a, tl.g).base) + tl.m0;
         const int slab = a.offsets != nullptr ? 0 : tl.g;
         for (int kb = 0; kb < KB; ++kb, ++it) {
           const int s = it % kStages;
-          if (!wait_blk(&empty[s], ((it / kStages) & 1u) ^ 1u, a, &s_abort)) break;
+          ok = wait_blk(&empty[s], ((it / kStages) & 1u) ^ 1u, a, &s_abort);
+          if (!ok) break;
           if (elect_one()) {
             mbar_arrive_expect_tx(&full[s], kStageBytes);
             tma_load_3d(sA + s * kABytes, &tmA, &full[s], kb * kBK, row, slab);
@@ -425,16 +429,19 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       const uint32_t b = warp - 1;
       constexpr uint32_t idesc = idesc_fp8(kBN, false, B_MN);
       uint32_t it = 0;
+      bool ok = true;
       BlkTile tl;
-      for (int t = blockIdx.x; !s_abort && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
+      for (int t = blockIdx.x; ok && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
         for (int kb = 0; kb < KB; ++kb, ++it) {
           if ((it & 1u) != b) continue;
           const int s = it % kStages;
           // the buffer comes last: from its release on every cycle delays the next block
-          if (!wait_blk(&full[s], (it / kStages) & 1u, a, &s_abort)) break;
+          ok = wait_blk(&full[s], (it / kStages) & 1u, a, &s_abort);
+          if (!ok) break;
           const uint64_t ad = smem_desc_k128(sA + s * kABytes);
           const uint64_t bd = B_MN ? smem_desc_mn128(sB + s * kBBytes, 128 * kBK) : smem_desc_k128(sB + s * kBBytes);
-          if (!wait_blk(&tempty[b], ((it >> 1) & 1u) ^ 1u, a, &s_abort)) break;
+          ok = wait_blk(&tempty[b], ((it >> 1) & 1u) ^ 1u, a, &s_abort);
+          if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
             // next 32 channels: 32 bytes along a K-major swizzle row, or 32 rows of 128 bytes
@@ -487,7 +494,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       uint32_t it = 0, u = 0;
       bool ok = true;
       BlkTile at;
-      for (int tt = blockIdx.x; ok && !s_abort && blk_tile(tt, a, s_grp, at); tt += gridDim.x) {
+      for (int tt = blockIdx.x; ok && blk_tile(tt, a, s_grp, at); tt += gridDim.x) {
         for (int kb = 0; kb < KB && ok; ++kb, ++it) {
           const int s = u & 1, j = kb & 3, b = it & 1;
           if (j == 0) {
@@ -704,14 +711,16 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     uint32_t it = 0;
+    bool ok = true;
     FewTiles f(a, s_grp, crank, csize);
-    while (!s_abort && f.advance()) {
+    while (ok && f.advance()) {
       const BlkTile tl = f.tl;
       const int row = static_cast<int>(f.sp.base) + tl.m0;
       const int slab = a.offsets != nullptr ? 0 : tl.g;
       for (int kb = f.k0; kb < f.k1; ++kb, ++it) {
         const int s = it % kFewStages;
-        if (!wait_blk(&fempty[s], ((it / kFewStages) & 1u) ^ 1u, a, &s_abort)) break;
+        ok = wait_blk(&fempty[s], ((it / kFewStages) & 1u) ^ 1u, a, &s_abort);
+        if (!ok) break;
         if (elect_one()) {
           mbar_arrive_expect_tx(&ffull[s], kFewStageBytes);
           uint8_t* db = smem + s * kFewStageBytes;
@@ -734,16 +743,19 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
     uint32_t it = 0;
+    bool ok = true;
     FewTiles f(a, s_grp, crank, csize);
-    while (!s_abort && f.advance()) {
+    while (ok && f.advance()) {
       const int n = (min(f.sp.cnt - f.tl.m0, kFewTile) + 15) / 16 * 16;
       const uint32_t idesc = idesc_fp8(n, B_MN, false);
       for (int kb = f.k0; kb < f.k1; ++kb, ++it) {
         const int s = it % kFewStages, b = it % kFewBufs;
-        if (!wait_blk(&ffull[s], (it / kFewStages) & 1u, a, &s_abort)) break;
+        ok = wait_blk(&ffull[s], (it / kFewStages) & 1u, a, &s_abort);
+        if (!ok) break;
         const uint8_t* db = smem + s * kFewStageBytes;
         const uint64_t xd = smem_desc_k128(db + kBBytes);
-        if (!wait_blk(&ftempty[b], ((it / kFewBufs) & 1u) ^ 1u, a, &s_abort)) break;
+        ok = wait_blk(&ftempty[b], ((it / kFewBufs) & 1u) ^ 1u, a, &s_abort);
+        if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
           constexpr uint64_t wstep = B_MN ? (32 * 128) >> 4 : 2;
@@ -793,7 +805,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
     uint32_t it = 0, u = 0;
     bool ok = true;
     FewTiles f(a, s_grp, crank, csize);
-    while (ok && !s_abort && f.advance()) {
+    while (ok && f.advance()) {
       for (int kb = f.k0; kb < f.k1 && ok; ++kb, ++it) {
         const int s = u & 1, j = (kb - f.k0) & 3, b = it % kFewBufs;
         if (j == 0) {
