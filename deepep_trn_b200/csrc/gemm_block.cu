@@ -137,6 +137,10 @@ template <int BYTES>
 __device__ __forceinline__ void cp_async(void* smem, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(src), "n"(BYTES) : "memory");
 }
+__device__ __forceinline__ void give_up(const BlkArgs& a, volatile int* abort) {
+  atomicExch(a.error, 1u);
+  *abort = 1;
+}
 // Bounded wait of a whole warp, whose lanes leave it together with one answer: what follows (elect.sync, TMEM
 // loads, barriers) needs all of them. The clock and the abort flag are looked at once in 256 polls, of which
 // each is suspended for up to 4 us. Every hand-over between warps through an mbarrier takes about 130 cycles;
@@ -149,12 +153,18 @@ __device__ __forceinline__ bool wait_blk(uint64_t* bar, uint32_t parity, const B
       const uint64_t now = global_ns();
       if (t0 == 0) t0 = now;
       if (__any_sync(0xffffffffu, *abort || now - t0 > a.timeout_ns)) {
-        atomicExch(a.error, 1u);
-        *abort = 1;
+        give_up(a, abort);
         return false;
       }
     }
   }
+}
+// The copies of the last STAGES of `it` blocks land before the CTA gives up its shared memory, whichever warp
+// gave up waiting for them (otherwise they have been used, and nothing is left to wait for).
+template <int STAGES>
+__device__ __forceinline__ void land_copies(uint64_t* full, uint32_t it) {
+  for (uint32_t q = it > STAGES ? it - STAGES : 0; q < it; ++q)
+    mbar_wait(&full[q % STAGES], (q / STAGES) & 1u, 1000000000ull);
 }
 
 struct Groups {
@@ -418,10 +428,7 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
           __syncwarp();
         }
       }
-      if (s_abort) {  // copies in flight land before the CTA's shared memory is given up
-        for (uint32_t q = it > kStages ? it - kStages : 0; q < it; ++q)
-          mbar_wait(&full[q % kStages], (q / kStages) & 1u, 1000000000ull);
-      }
+      land_copies<kStages>(full, it);
     } else if (warp <= 2) {
       // ------------------------------------------------------------------ MMA issuers
       // one warp for each TMEM buffer: the waits and the issue of a K block's MMAs take one warp
@@ -429,7 +436,8 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
       const uint32_t b = warp - 1;
       constexpr uint32_t idesc = idesc_fp8(kBN, false, B_MN);
       uint32_t it = 0;
-      bool ok = true;
+      bool ok = a.timeout_ns != 0;   // without a budget nothing is multiplied, and all that wait for it run out
+      if (!ok) give_up(a, &s_abort);
       BlkTile tl;
       for (int t = blockIdx.x; ok && blk_tile(t, a, s_grp, tl); t += gridDim.x) {
         for (int kb = 0; kb < KB; ++kb, ++it) {
@@ -736,14 +744,12 @@ __global__ void __launch_bounds__(kBlkThreads, 1)
         __syncwarp();
       }
     }
-    if (s_abort) {  // copies in flight land before the CTA's shared memory is given up
-      for (uint32_t q = it > kFewStages ? it - kFewStages : 0; q < it; ++q)
-        mbar_wait(&ffull[q % kFewStages], (q / kFewStages) & 1u, 1000000000ull);
-    }
+    land_copies<kFewStages>(ffull, it);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
     uint32_t it = 0;
-    bool ok = true;
+    bool ok = a.timeout_ns != 0;   // as in the other kernel
+    if (!ok) give_up(a, &s_abort);
     FewTiles f(a, s_grp, crank, csize);
     while (ok && f.advance()) {
       const int n = (min(f.sp.cnt - f.tl.m0, kFewTile) + 15) / 16 * 16;
@@ -1162,7 +1168,7 @@ void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at:
   a.sb_n = b_kn ? 1 : KB;
   a.sb_k = b_kn ? NB : 1;
   a.error = reinterpret_cast<uint32_t*>(error.data_ptr<int32_t>());
-  a.timeout_ns = static_cast<uint64_t>(timeout_s * 1e9);
+  a.timeout_ns = timeout_s > 0 ? static_cast<uint64_t>(std::min(timeout_s, 1e9) * 1e9) : 0;
   // a stride over a dimension of one element is arbitrary; the map wants a legal one
   auto stride = [](const at::Tensor& t, int64_t d, int64_t otherwise) { return t.size(d) > 1 ? t.stride(d) : otherwise; };
   const int64_t s1 = stride(A, A.dim() - 2, K);

@@ -165,6 +165,9 @@ def grouped_gemm_fp8_block(A, sa, B, sb, offsets=None, counts=None, out=None, ep
     (``interleave_gate_up``) and returns ``(h, h_scales, pre)``: ``h = silu(gate) * up`` in e4m3 with
     fp32 1x128 scales, the operand of the next product, and the bf16 pre-activation with
     ``save_preact`` (else None). ``out``, ``h_out``, ``h_scales`` receive C / pre, h and its scales.
+
+    ``timeout_s`` bounds each wait inside the kernels. One that runs out ends the call, whose output is then
+    not to be used, and ``check()`` raises (0: the call gives up without multiplying anything).
     """
     if epilogue not in FP8_BLOCK_EPILOGUES:
         raise ValueError(f'unknown epilogue {epilogue!r}; expected one of {tuple(FP8_BLOCK_EPILOGUES)}')
