@@ -25,7 +25,7 @@
 //               the output's extent); the accumulator is freed as soon as it has
 //               been read, so the stores overlap the next tile's MMAs.
 // Every mbarrier wait is bounded; on timeout the CTA records an error, stops
-// issuing, frees its TMEM and returns.
+// issuing, lets the copies in flight land, frees its TMEM and returns.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include "ops.h"
@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     a.sfb_tiles + ((static_cast<int64_t>(tl.g) * ntn + tl.n0 / BN) * KB + kg) * 512, 512, &full[s]);
         }
       }
+      land_copies<STAGES>(full, it);
     }
   } else if (!FP8 && warp == 0) {
     // ------------------------------------------------------------------ TMA producer
@@ -275,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      land_copies<STAGES>(full, it);
     }
   } else if (FP8 && warp == 1) {
     // ------------------------------------------------------------------ MMA issuer (fp8, block-scaled)
@@ -282,6 +284,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc = idesc_fp8_bs(BN);
       constexpr uint32_t kSfCol0 = 2 * BN;   // scale columns follow the two accumulators
       uint32_t it = 0, acc = 0;
+      if (a.timeout_ns == 0) {   // without a budget nothing is multiplied, and all that wait for it run out
+        atomicExch(a.error, 1u);
+        s_abort = 1;
+      }
       Tile tl;
       for (int t = blockIdx.x; tile_of<GROUP_K, BN, KBLK>(t, a, s_offs, tl) && !s_abort; t += gridDim.x) {
         if (tl.nkb == 0) continue;
@@ -321,6 +327,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_bf16(BN, A_MN, B_MN);
       uint32_t it = 0, acc = 0;
+      if (a.timeout_ns == 0) {   // without a budget nothing is multiplied, and all that wait for it run out
+        atomicExch(a.error, 1u);
+        s_abort = 1;
+      }
       Tile tl;
       for (int t = blockIdx.x; tile_of<GROUP_K, BN>(t, a, s_offs, tl) && !s_abort; t += gridDim.x) {
         if (tl.nkb == 0) continue;  // empty expert: the epilogue writes zeros without the accumulator
@@ -381,8 +391,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = acc & 1;
       const bool have = tl.nkb > 0;
       if (have) {
-        if (!wait_bar(&tfull[b], (acc >> 1) & 1u, a)) { s_abort = 1; }
-        if (s_abort) break;
+        // a warp leaves with one answer: the TMEM loads need all of its lanes
+        if (!__all_sync(0xffffffffu, wait_bar(&tfull[b], (acc >> 1) & 1u, a) && !s_abort)) {
+          s_abort = 1;
+          break;
+        }
         tc_fence_after();
       }
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * BN;
@@ -578,7 +591,7 @@ void grouped_gemm_m(const at::Tensor& A, const at::Tensor& B, const at::Tensor& 
   TORCH_CHECK(!b_kn || a.N % 64 == 0, "an MN-major B needs N % 64 == 0");
   a.offsets = offsets.data_ptr<int64_t>();
   a.error = reinterpret_cast<uint32_t*>(error.data_ptr<int32_t>());
-  a.timeout_ns = static_cast<uint64_t>(timeout_s * 1e9);
+  a.timeout_ns = timeout_ns(timeout_s);
   const CUtensorMap ma = make_map(A.data_ptr(), A.size(0), a.K, A.stride(0), BM);
   const CUtensorMap mb = b_kn ? make_map_kn(B.data_ptr(), a.G, a.K, a.N)
                               : make_map(B.data_ptr(), int64_t(a.G) * a.N, a.K, a.K, 256);
@@ -644,7 +657,7 @@ void grouped_gemm_k(const at::Tensor& A, const at::Tensor& B, const at::Tensor& 
   a.ldc = a.N;
   a.c_group_stride = int64_t(a.M) * a.N;
   a.error = reinterpret_cast<uint32_t*>(error.data_ptr<int32_t>());
-  a.timeout_ns = static_cast<uint64_t>(timeout_s * 1e9);
+  a.timeout_ns = timeout_ns(timeout_s);
   // token-major: boxes of 64 (M or N) x BK tokens, one per 64-wide MN atom
   const CUtensorMap ma = tok_major ? make_map(A.data_ptr(), A.size(0), a.M, A.stride(0), BK)
                                    : make_map(A.data_ptr(), a.M, A.size(1), A.stride(0), BM);
@@ -737,7 +750,7 @@ void grouped_gemm_fp8_m(const at::Tensor& A, const at::Tensor& sa, const at::Ten
   a.sfb_tiles = tb.data_ptr<uint8_t>();
   a.offsets = offsets.data_ptr<int64_t>();
   a.error = reinterpret_cast<uint32_t*>(error.data_ptr<int32_t>());
-  a.timeout_ns = static_cast<uint64_t>(timeout_s * 1e9);
+  a.timeout_ns = timeout_ns(timeout_s);
   constexpr int BN8 = 128;
   const CUtensorMap ma = make_map_u8(A.data_ptr(), A.size(0), a.K, A.stride(0), BM);
   const CUtensorMap mb = make_map_u8(B.data_ptr(), int64_t(a.G) * a.N, a.K, a.K, BN8);

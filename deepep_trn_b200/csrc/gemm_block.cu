@@ -159,13 +159,6 @@ __device__ __forceinline__ bool wait_blk(uint64_t* bar, uint32_t parity, const B
     }
   }
 }
-// The copies of the last STAGES of `it` blocks land before the CTA gives up its shared memory, whichever warp
-// gave up waiting for them (otherwise they have been used, and nothing is left to wait for).
-template <int STAGES>
-__device__ __forceinline__ void land_copies(uint64_t* full, uint32_t it) {
-  for (uint32_t q = it > STAGES ? it - STAGES : 0; q < it; ++q)
-    mbar_wait(&full[q % STAGES], (q / STAGES) & 1u, 1000000000ull);
-}
 
 struct Groups {
   int pref[kMaxG + 1];   // tiles (of rows) of the groups before; none for a group of the other form
@@ -1168,7 +1161,7 @@ void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at:
   a.sb_n = b_kn ? 1 : KB;
   a.sb_k = b_kn ? NB : 1;
   a.error = reinterpret_cast<uint32_t*>(error.data_ptr<int32_t>());
-  a.timeout_ns = timeout_s > 0 ? static_cast<uint64_t>(std::min(timeout_s, 1e9) * 1e9) : 0;
+  a.timeout_ns = timeout_ns(timeout_s);
   // a stride over a dimension of one element is arbitrary; the map wants a legal one
   auto stride = [](const at::Tensor& t, int64_t d, int64_t otherwise) { return t.size(d) > 1 ? t.stride(d) : otherwise; };
   const int64_t s1 = stride(A, A.dim() - 2, K);

@@ -157,6 +157,14 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&p);
 }
 
+// The copies of the last STAGES of `it` blocks land before the CTA gives up its shared memory, whichever warp
+// gave up waiting for them (otherwise they have been used, and nothing is left to wait for).
+template <int STAGES>
+__device__ __forceinline__ void land_copies(uint64_t* full, uint32_t it) {
+  for (uint32_t q = it > STAGES ? it - STAGES : 0; q < it; ++q)
+    mbar_wait(&full[q % STAGES], (q / STAGES) & 1u, 1000000000ull);
+}
+
 // ----------------------------------------------------------------------------- host side
 using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
 
@@ -170,6 +178,11 @@ inline EncodeFn encoder() {
     fn = reinterpret_cast<EncodeFn>(p);
   }
   return fn;
+}
+
+// The budget of a wait; what is not above zero (a NaN too) is none.
+inline uint64_t timeout_ns(double seconds) {
+  return seconds > 0 ? static_cast<uint64_t>(std::min(seconds, 1e9) * 1e9) : 0;
 }
 
 }  // namespace gemm
