@@ -88,6 +88,37 @@ __host__ __device__ inline int64_t few_cycles(int64_t tiles, int64_t KB, int64_t
          rounds * ((KB + split - 1) / split * block_cycles(left * split, grid, true) + 6000) + 4000;
 }
 
+// The groups of a call with slabs: tiles as many rows, as few, and with each group in the form that its rows
+// suggest; groups with rows.
+struct Tally {
+  int many, few, many_part, few_part, busy;
+  __host__ __device__ void add(int n) {
+    const int m = (n + kBM - 1) / kBM, f = (n + kFewTile - 1) / kFewTile;
+    many += m;
+    few += f;
+    (f > 1 ? many_part : few_part) += f > 1 ? m : f;
+    busy += n > 0;
+  }
+};
+// The launches of a call. Both kernels are given the same, and conclude the same from it.
+struct Plan {
+  int form;                 // Form
+  int sms;                  // SMs that the call may use
+  int split, few_grid;      // kernel for few rows: CTAs of a cluster that divide K, CTAs
+  int many_grid;            // kernel for many rows: CTAs
+  bool overlap;             // the second kernel starts while the first still runs
+};
+// The most rows of a group that counts as one with few, where both kernels are launched: all groups as many,
+// all as few, or each by its rows, whichever has the least estimate.
+__host__ __device__ inline int few_rows_of(const Tally& t, int64_t N, int64_t K, const Plan& p) {
+  const int64_t ntn = (N + kBN - 1) / kBN, KB = (K + kBK - 1) / kBK;
+  const int64_t as_many = many_cycles(t.many * ntn, KB, p.sms, t.many == t.busy);
+  const int64_t as_few = few_cycles(t.few * ntn, KB, p.few_grid, p.split);
+  const int64_t mixed = few_cycles(t.few_part * ntn, KB, p.few_grid, p.split) +
+                        many_cycles(t.many_part * ntn, KB, p.sms, t.many_part == t.busy - t.few_part);
+  return as_few <= (as_many < mixed ? as_many : mixed) ? INT_MAX : mixed < as_many ? kFewTile : 0;
+}
+
 struct BlkArgs {
   const int64_t* offsets;   // [G + 1] or nullptr (masked)
   const int32_t* counts;    // [G] or nullptr
@@ -104,8 +135,7 @@ struct BlkArgs {
   int64_t hs_row, hs_group;
   uint32_t* error;
   uint64_t timeout_ns;
-  int form;                 // Form
-  int sms, split, few_grid; // launch shapes, from which both kernels conclude the same
+  Plan plan;
 };
 
 __device__ __forceinline__ void tc_mma_fp8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -191,28 +221,16 @@ __device__ __forceinline__ void load_groups(Groups& s, const BlkArgs& a) {
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int few_rows = a.form == kAllFew ? INT_MAX : 0;   // most rows of a group that counts as one with few
-    if (a.form == kBothForms) {
-      // all groups as many, all as few, or each by its rows: the least estimate
-      int many = 0, few = 0, many_part = 0, few_part = 0, busy = 0;
-      for (int g = lane; g < a.G; g += 32) {
-        const int n = s.pref[g + 1], m = (n + kBM - 1) / kBM, f = (n + kFewTile - 1) / kFewTile;
-        many += m;
-        few += f;
-        (f > 1 ? many_part : few_part) += f > 1 ? m : f;
-        busy += n > 0;
-      }
-      many = __reduce_add_sync(0xffffffffu, many);
-      few = __reduce_add_sync(0xffffffffu, few);
-      many_part = __reduce_add_sync(0xffffffffu, many_part);
-      few_part = __reduce_add_sync(0xffffffffu, few_part);
-      busy = __reduce_add_sync(0xffffffffu, busy);
-      const int64_t ntn = (a.N + kBN - 1) / kBN, KB = (a.K + kBK - 1) / kBK;
-      const int64_t as_many = many_cycles(many * ntn, KB, a.sms, many == busy);
-      const int64_t as_few = few_cycles(few * ntn, KB, a.few_grid, a.split);
-      const int64_t mixed = few_cycles(few_part * ntn, KB, a.few_grid, a.split) +
-                            many_cycles(many_part * ntn, KB, a.sms, many_part == busy - few_part);
-      few_rows = as_few <= min(as_many, mixed) ? INT_MAX : mixed < as_many ? kFewTile : 0;
+    int few_rows = a.plan.form == kAllFew ? INT_MAX : 0;   // most rows of a group that counts as one with few
+    if (a.plan.form == kBothForms) {
+      Tally t{};
+      for (int g = lane; g < a.G; g += 32) t.add(s.pref[g + 1]);
+      t.many = __reduce_add_sync(0xffffffffu, t.many);
+      t.few = __reduce_add_sync(0xffffffffu, t.few);
+      t.many_part = __reduce_add_sync(0xffffffffu, t.many_part);
+      t.few_part = __reduce_add_sync(0xffffffffu, t.few_part);
+      t.busy = __reduce_add_sync(0xffffffffu, t.busy);
+      few_rows = few_rows_of(t, a.N, a.K, a.plan);
     }
     int total = 0;
     for (int g0 = 0; g0 < a.G; g0 += 32) {
@@ -983,77 +1001,98 @@ CUtensorMap map_u8_3d(const void* base, int64_t d0, int64_t d1, int64_t d2, int6
   return m;
 }
 
-// The kernel for groups with few rows in clusters of `split`; grid 0: the CTAs that are resident together
-// (a GPC's SMs need not divide into clusters) is asked for, once for each size.
+// The kernel for groups with few rows in clusters of `split`.
 template <int EPI, bool B_MN>
-int few_launch(const CUtensorMap& ma, const CUtensorMap& mb, const BlkArgs& a, int grid, int split, cudaStream_t stream) {
-  constexpr int smem = 1024 + kFewStages * kFewStageBytes + kFewTile * kBN * 4;
-  auto kfn = gemm_few_kernel<EPI, B_MN>;
-  static std::atomic<uint64_t> seen{0};
-  AT_CUDA_CHECK(set_smem_limit_once(seen, kfn, smem));
+struct FewLaunch {
+  static constexpr int kSmem = 1024 + kFewStages * kFewStageBytes + kFewTile * kBN * 4;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid > 0 ? grid : split);
-  cfg.blockDim = dim3(kBlkThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
   cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = split;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = split > 1 ? 1 : 0;
-  if (grid == 0) {
-    if (split == 1) return a.sms;
-    static std::atomic<int> resident[kMaxSplit + 1] = {};
-    int clusters = resident[split].load(std::memory_order_relaxed);
-    if (clusters == 0) {
-      AT_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, kfn, &cfg));
-      TORCH_CHECK(clusters > 0, "no cluster of the fp8 GEMM fits on this device");
-      resident[split].store(clusters, std::memory_order_relaxed);
-    }
-    return std::max(1, std::min(clusters, a.sms / split)) * split;
+  FewLaunch(int grid, int split, cudaStream_t stream) {
+    static std::atomic<uint64_t> seen{0};
+    AT_CUDA_CHECK(set_smem_limit_once(seen, gemm_few_kernel<EPI, B_MN>, kSmem));
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kBlkThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
   }
-  AT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kfn, ma, mb, a));
-  return grid;
+  FewLaunch(const FewLaunch&) = delete;
+};
+// The clusters of `split` CTAs that are resident together (a GPC's SMs need not divide into clusters), asked
+// for once for each size.
+template <int EPI, bool B_MN>
+int resident_clusters(int split) {
+  static std::atomic<int> resident[kMaxSplit + 1] = {};
+  int clusters = resident[split].load(std::memory_order_relaxed);
+  if (clusters == 0) {
+    const FewLaunch<EPI, B_MN> l(split, split, nullptr);
+    AT_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, gemm_few_kernel<EPI, B_MN>, &l.cfg));
+    TORCH_CHECK(clusters > 0, "no cluster of the fp8 GEMM fits on this device");
+    resident[split].store(clusters, std::memory_order_relaxed);
+  }
+  return clusters;
 }
 
-// One call: the forms that its rows take, and the launches. `rows_known`: the rows of all groups together
-// (an upper bound), or 0 where only the device knows (slabs).
-template <int EPI, bool B_MN>
-void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMap& mb, BlkArgs a, int64_t rows_known,
-                  cudaStream_t stream) {
-  const int64_t ntn = (a.N + kBN - 1) / kBN, KB = (a.K + kBK - 1) / kBK;
+// The forms that a call's rows take, and the launches, for a call that may use `sms` of a device's `all` SMs.
+// rows: of all groups together (segments; an upper bound), or of a slab, whose counts only the device knows.
+// clusters(split): clusters of that size that are resident together.
+template <typename Clusters>
+Plan make_plan(int64_t G, int64_t rows, int64_t N, int64_t K, bool masked, int sms, int all, Clusters clusters) {
+  Plan p{};
+  p.sms = sms;
+  const int64_t ntn = (N + kBN - 1) / kBN, KB = (K + kBK - 1) / kBK;
   // tiles of groups with few rows: one a group (slabs), or as many as the rows make
-  const int64_t some = std::min<int64_t>(a.G, rows_known);
-  const int64_t few = (rows_known == 0 ? a.G : std::max<int64_t>(some, (rows_known + kFewTile - 1) / kFewTile)) * ntn;
+  const int64_t some = std::min(G, rows);
+  const int64_t few = (masked ? G : std::max(some, (rows + kFewTile - 1) / kFewTile)) * ntn;
   int64_t least = -1;
-  for (int s = 1; s <= kMaxSplit && s * 2 <= std::max<int64_t>(KB, 2) && s <= a.sms; s *= 2) {
-    const int grid = few_launch<EPI, B_MN>(ma, mb, a, 0, s, stream);
+  for (int s = 1; s <= kMaxSplit && s * 2 <= std::max<int64_t>(KB, 2) && s <= sms; s *= 2) {
+    const int grid = s == 1 ? sms : std::max(1, std::min(clusters(s), sms / s)) * s;
     const int64_t cycles = few_cycles(few, KB, grid, s);
     if (least < 0 || cycles < least) {
       least = cycles;
-      a.split = s;
-      a.few_grid = grid;
+      p.split = s;
+      p.few_grid = grid;
     }
   }
-  if (rows_known > 0) {
-    a.few_grid = static_cast<int>(std::min<int64_t>(a.few_grid, few * a.split));   // no CTA without work
+  p.many_grid = sms;
+  if (!masked) {
+    p.few_grid = static_cast<int>(std::min<int64_t>(p.few_grid, few * p.split));   // no CTA without work
     // half a tile more a group than its rows fill, on average, and at least one
-    const int64_t many = std::max<int64_t>(some, (rows_known + kBM - 1) / kBM + some / 2) * ntn;
-    a.form = least < many_cycles(many, KB, a.sms, many == some * ntn) ? kAllFew : kAllMany;
-    a.sms = static_cast<int>(std::min<int64_t>(a.sms, many));
+    const int64_t many = std::max<int64_t>(some, (rows + kBM - 1) / kBM + some / 2) * ntn;
+    p.form = least < many_cycles(many, KB, sms, many == some * ntn) ? kAllFew : kAllMany;
+    p.many_grid = static_cast<int>(std::min<int64_t>(sms, many));
   } else {
     // a decoding step, a tile a group, decides whether the form for few rows is worth its launch
-    a.form = least >= many_cycles(few, KB, a.sms, true) ? kAllMany : a.rows <= kFewTile ? kAllFew : kBothForms;
+    p.form = least >= many_cycles(few, KB, sms, true) ? kAllMany : rows <= kFewTile ? kAllFew : kBothForms;
   }
-  if (a.form != kAllMany) few_launch<EPI, B_MN>(mf, mb, a, a.few_grid, a.split, stream);
-  if (a.form == kAllFew) return;
+  // side by side the two kernels may hold twice `sms` SMs, which a caller that keeps some back must not see
+  p.overlap = p.form == kBothForms && sms >= all;
+  return p;
+}
+
+int granted_sms(int64_t num_sms, int all) { return num_sms > 0 ? static_cast<int>(std::min<int64_t>(num_sms, all)) : all; }
+
+template <int EPI, bool B_MN>
+void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMap& mb, BlkArgs a, bool masked,
+                  int64_t num_sms, cudaStream_t stream) {
+  const int all = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const Plan& p = a.plan =
+      make_plan(a.G, a.rows, a.N, a.K, masked, granted_sms(num_sms, all), all, resident_clusters<EPI, B_MN>);
+  if (p.form != kAllMany) {
+    const FewLaunch<EPI, B_MN> l(p.few_grid, p.split, stream);
+    AT_CUDA_CHECK(cudaLaunchKernelEx(&l.cfg, gemm_few_kernel<EPI, B_MN>, mf, mb, a));
+  }
+  if (p.form == kAllFew) return;
   constexpr int smem = 1024 + kStages * kStageBytes + kEpiWarps * kWarpStage;
   auto kfn = gemm_block_kernel<EPI, B_MN>;
   static std::atomic<uint64_t> seen{0};
   AT_CUDA_CHECK(set_smem_limit_once(seen, kfn, smem));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(a.sms);
+  cfg.gridDim = dim3(p.many_grid);
   cfg.blockDim = dim3(kBlkThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -1061,7 +1100,7 @@ void launch_block(const CUtensorMap& ma, const CUtensorMap& mf, const CUtensorMa
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = a.form == kBothForms ? 1 : 0;
+  cfg.numAttrs = p.overlap ? 1 : 0;
   AT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kfn, ma, mb, a));
 }
 
@@ -1171,15 +1210,37 @@ void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at:
                                 : map_u8_3d(A.data_ptr(), K, a.rows, 1, s1, s1 * a.rows, kFewTile);
   const CUtensorMap mb = b_kn ? map_u8_3d(B.data_ptr(), N, K, a.G, N, N * K, kBK)
                               : map_u8_3d(B.data_ptr(), K, N, a.G, K, N * K, kBN);
-  const int all = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  a.sms = num_sms > 0 ? static_cast<int>(std::min<int64_t>(num_sms, all)) : all;
-  const int64_t known = masked ? 0 : a.rows;
   auto stream = at::cuda::getCurrentCUDAStream();
-  if (epilogue == kOutSwiGLU) launch_block<kOutSwiGLU, false>(ma, mf, mb, a, known, stream);
-  else if (epilogue == kOutBF16 && b_kn) launch_block<kOutBF16, true>(ma, mf, mb, a, known, stream);
-  else if (epilogue == kOutBF16) launch_block<kOutBF16, false>(ma, mf, mb, a, known, stream);
-  else if (b_kn) launch_block<kOutF32, true>(ma, mf, mb, a, known, stream);
-  else launch_block<kOutF32, false>(ma, mf, mb, a, known, stream);
+  if (epilogue == kOutSwiGLU) launch_block<kOutSwiGLU, false>(ma, mf, mb, a, masked, num_sms, stream);
+  else if (epilogue == kOutBF16 && b_kn) launch_block<kOutBF16, true>(ma, mf, mb, a, masked, num_sms, stream);
+  else if (epilogue == kOutBF16) launch_block<kOutBF16, false>(ma, mf, mb, a, masked, num_sms, stream);
+  else if (b_kn) launch_block<kOutF32, true>(ma, mf, mb, a, masked, num_sms, stream);
+  else launch_block<kOutF32, false>(ma, mf, mb, a, masked, num_sms, stream);
+}
+
+std::tuple<std::string, int64_t, int64_t, int64_t, bool> fp8_block_plan(
+    int64_t G, int64_t rows, int64_t N, int64_t K, bool masked, int64_t num_sms,
+    const c10::optional<std::vector<int64_t>>& counts, const c10::optional<std::vector<int64_t>>& device) {
+  using namespace gemm;
+  TORCH_CHECK(G >= 1 && rows >= 1 && N >= 1 && K >= 1, "sizes above zero");
+  Plan p;
+  if (device.has_value()) {   // SMs, and resident clusters of 2, 4 and 8 CTAs
+    TORCH_CHECK(device->size() == 4 && device->at(0) >= 1, "a device is its SMs and its resident clusters of 2, 4 and 8 CTAs");
+    const int all = static_cast<int>(device->at(0));
+    p = make_plan(G, rows, N, K, masked, granted_sms(num_sms, all), all,
+                  [&](int s) { return static_cast<int>(device->at(s == 2 ? 1 : s == 4 ? 2 : 3)); });
+  } else {
+    const int all = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    p = make_plan(G, rows, N, K, masked, granted_sms(num_sms, all), all, resident_clusters<kOutBF16, false>);
+  }
+  std::string form = p.form == kAllMany ? "many" : p.form == kAllFew ? "few" : "both";
+  if (p.form == kBothForms && counts.has_value()) {
+    Tally t{};
+    for (const int64_t n : *counts) t.add(static_cast<int>(std::max<int64_t>(0, std::min(n, rows))));
+    const int few_rows = few_rows_of(t, N, K, p);
+    form = few_rows == INT_MAX ? "both: few" : few_rows == 0 ? "both: many" : "both: mixed";
+  }
+  return {form, p.split, p.form == kAllMany ? 0 : p.few_grid, p.form == kAllFew ? 0 : p.many_grid, p.overlap};
 }
 
 }  // namespace b200ep

@@ -132,6 +132,13 @@ void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at:
                             const OptTensor& Hs, int64_t epilogue, const at::Tensor& error, int64_t num_sms,
                             double timeout_s, bool b_kn);
 
+// The launches of such a call: form ("few", "many", "both", with counts "both: ..."), cluster size, CTAs of the
+// kernels for few and for many rows, whether they overlap. device: SMs and resident clusters of 2, 4 and 8 CTAs of
+// a device that is not asked itself.
+std::tuple<std::string, int64_t, int64_t, int64_t, bool> fp8_block_plan(
+    int64_t G, int64_t rows, int64_t N, int64_t K, bool masked, int64_t num_sms,
+    const c10::optional<std::vector<int64_t>>& counts, const c10::optional<std::vector<int64_t>>& device);
+
 // gate.cu
 std::tuple<at::Tensor, at::Tensor> router_gate(const at::Tensor& logits, int64_t topk, bool sigmoid,
                                                const OptTensor& bias, int64_t num_groups, int64_t topk_groups,

@@ -166,6 +166,7 @@ def grouped_gemm_fp8_block(A, sa, B, sb, offsets=None, counts=None, out=None, ep
     fp32 1x128 scales, the operand of the next product, and the bf16 pre-activation with
     ``save_preact`` (else None). ``out``, ``h_out``, ``h_scales`` receive C / pre, h and its scales.
 
+    ``num_sms`` > 0 bounds the SMs that the call's kernels hold at a time (they then run one after the other).
     ``timeout_s`` bounds each wait inside the kernels. One that runs out ends the call, whose output is then
     not to be used, and ``check()`` raises (0: the call gives up without multiplying anything).
     """
@@ -191,6 +192,17 @@ def grouped_gemm_fp8_block(A, sa, B, sb, offsets=None, counts=None, out=None, ep
     if not A.is_cuda:
         _grouped_gemm_fp8_block_cpu(A, sa, B, sb, offsets, counts, c, h, hs, kn)
     return c if epilogue != 'swiglu' else (h, hs, c)
+
+
+def fp8_block_plan(G: int, rows: int, N: int, K: int, masked: bool, num_sms: int = 0, counts=None, device=None):
+    """What a ``grouped_gemm_fp8_block`` call of these sizes launches, as a dict: ``form`` ('few' or 'many' rows a
+    group, or 'both', where the device decides by the counts; with ``counts`` 'both: few', 'both: many' or
+    'both: mixed'), ``split`` (CTAs that divide K in the form for few rows), ``few_ctas``, ``many_ctas`` and
+    ``overlap`` (whether the kernels run side by side). ``rows`` are those of a slab (``masked``) or of all
+    segments. ``device`` gives the SMs and the resident clusters of 2, 4 and 8 CTAs of a device other than the
+    current one. The kernels together hold no more SMs than ``num_sms`` grants."""
+    plan = load().fp8_block_plan(G, rows, N, K, masked, num_sms, counts, device)
+    return dict(zip(('form', 'split', 'few_ctas', 'many_ctas', 'overlap'), plan))
 
 
 def _grouped_gemm_fp8_block_cpu(A, sa, B, sb, offsets, counts, c, h, hs, kn):
