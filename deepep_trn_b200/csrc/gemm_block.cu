@@ -42,6 +42,7 @@
 
 #include <climits>
 
+#include "device_table.h"
 #include "ops.h"
 #include "tcgen05.cuh"
 
@@ -1022,19 +1023,18 @@ struct FewLaunch {
   }
   FewLaunch(const FewLaunch&) = delete;
 };
-// The clusters of `split` CTAs that are resident together (a GPC's SMs need not divide into clusters), asked
-// for once for each size.
+// The clusters of `split` CTAs that are resident together on the current device (a GPC's SMs need not divide
+// into clusters, and cards differ), asked for once for each device and size.
 template <int EPI, bool B_MN>
 int resident_clusters(int split) {
-  static std::atomic<int> resident[kMaxSplit + 1] = {};
-  int clusters = resident[split].load(std::memory_order_relaxed);
-  if (clusters == 0) {
+  static DeviceTable<kMaxSplit + 1> resident;
+  return resident.get(c10::cuda::current_device(), split, [split] {
+    int clusters = 0;
     const FewLaunch<EPI, B_MN> l(split, split, nullptr);
     AT_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&clusters, gemm_few_kernel<EPI, B_MN>, &l.cfg));
     TORCH_CHECK(clusters > 0, "no cluster of the fp8 GEMM fits on this device");
-    resident[split].store(clusters, std::memory_order_relaxed);
-  }
-  return clusters;
+    return clusters;
+  });
 }
 
 // The forms that a call's rows take, and the launches, for a call that may use `sms` of a device's `all` SMs.
