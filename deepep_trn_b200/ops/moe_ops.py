@@ -57,11 +57,16 @@ def router_gate(logits: torch.Tensor, k: int, scoring: str = 'sigmoid', bias: to
     A logit of -inf or NaN (or a bias of -inf) makes an expert unavailable. Where fewer than k
     are available the remaining ids are -1 with weight 0, which ``dispatch`` skips. +inf counts
     as the largest finite value. E <= 1024, k <= 32, num_groups <= 32.
+
+    The weights are differentiable once in the logits (by ``router_gate_bwd``), the selection and the bias
+    are not.
     """
     if scoring not in ('sigmoid', 'softmax'):
         raise ValueError(f"unknown scoring {scoring!r}; expected 'sigmoid' or 'softmax'")
     if group_score not in ('top2', 'max'):
         raise ValueError(f"unknown group_score {group_score!r}; expected 'top2' or 'max'")
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _RouterGate.apply(logits, k, scoring, bias, num_groups, topk_groups, group_score, renormalize, scale)
     if not logits.is_cuda:
         if available():   # the argument checks
             load().router_gate(logits, k, scoring == 'sigmoid', bias, num_groups, topk_groups, group_score == 'top2',
@@ -69,6 +74,22 @@ def router_gate(logits: torch.Tensor, k: int, scoring: str = 'sigmoid', bias: to
         return router_gate_reference(logits, k, scoring, bias, num_groups, topk_groups, group_score, renormalize, scale)
     return load().router_gate(logits, k, scoring == 'sigmoid', bias, num_groups, topk_groups, group_score == 'top2',
                               renormalize, scale)
+
+
+class _RouterGate(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, scoring, bias, num_groups, topk_groups, group_score, renormalize, scale):
+        idx, w = router_gate(logits, k, scoring, bias, num_groups, topk_groups, group_score, renormalize, scale)
+        ctx.mark_non_differentiable(idx)
+        ctx.save_for_backward(logits, idx)
+        ctx.args = scoring, renormalize, scale
+        return idx, w
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, _, dw):
+        logits, idx = ctx.saved_tensors
+        return (router_gate_bwd(logits, idx, dw, *ctx.args),) + (None,) * 8
 
 
 def router_gate_bwd(logits: torch.Tensor, idx: torch.Tensor, dw: torch.Tensor, scoring: str = 'sigmoid',
