@@ -589,6 +589,7 @@ void grouped_gemm_m(const at::Tensor& A, const at::Tensor& B, const at::Tensor& 
   a.M = static_cast<int>(A.size(0));
   TORCH_CHECK(A.size(1) == a.K && a.K % 8 == 0, "K mismatch / K % 8");
   TORCH_CHECK(!b_kn || a.N % 64 == 0, "an MN-major B needs N % 64 == 0");
+  if (A.size(0) == 0) return;   // (a tensor map has no empty side)
   a.offsets = offsets.data_ptr<int64_t>();
   a.error = reinterpret_cast<uint32_t*>(error.data_ptr<int32_t>());
   a.timeout_ns = timeout_ns(timeout_s);
@@ -652,6 +653,11 @@ void grouped_gemm_k(const at::Tensor& A, const at::Tensor& B, const at::Tensor& 
   TORCH_CHECK(!tok_major || (a.M % 64 == 0 && a.N % 64 == 0 && A.size(0) == B.size(0)),
               "token-major operands need M, N multiples of 64 and the same token count");
   TORCH_CHECK(C.size(1) == a.M && C.size(2) == a.N && offsets.numel() == a.G + 1 && a.G <= 1024, "shape mismatch");
+  TORCH_CHECK(C.scalar_type() == at::kFloat || C.scalar_type() == at::kBFloat16, "C must be fp32 or bf16");
+  if (A.size(tok_major ? 0 : 1) == 0) {   // the sums over no tokens
+    C.zero_();
+    return;
+  }
   a.offsets = offsets.data_ptr<int64_t>();
   a.C = C.data_ptr();
   a.ldc = a.N;
@@ -663,7 +669,6 @@ void grouped_gemm_k(const at::Tensor& A, const at::Tensor& B, const at::Tensor& 
                                    : make_map(A.data_ptr(), a.M, A.size(1), A.stride(0), BM);
   const CUtensorMap mb = tok_major ? make_map(B.data_ptr(), B.size(0), a.N, B.stride(0), BK)
                                    : make_map(B.data_ptr(), a.N, B.size(1), B.stride(0), 256);
-  TORCH_CHECK(C.scalar_type() == at::kFloat || C.scalar_type() == at::kBFloat16, "C must be fp32 or bf16");
   const bool f32 = C.scalar_type() == at::kFloat;
   const CUtensorMap mc = make_out_map(a.C, f32, a.M, a.N, a.N, a.G);
   const int sms = num_sms > 0 ? static_cast<int>(num_sms) : at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
@@ -733,6 +738,7 @@ void grouped_gemm_fp8_m(const at::Tensor& A, const at::Tensor& sa, const at::Ten
   a.K = static_cast<int>(B.size(2));
   a.M = static_cast<int>(A.size(0));
   TORCH_CHECK(A.size(1) == a.K && a.K % 128 == 0, "K mismatch, or K not a multiple of 128");
+  if (A.size(0) == 0) return;
   const int64_t KB = a.K / 128;
   TORCH_CHECK(sa.scalar_type() == at::kByte ||
                   (sa.scalar_type() == at::kFloat && sa.dim() == 2 && sa.size(0) == A.size(0) && sa.size(1) == KB &&
