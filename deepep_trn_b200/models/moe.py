@@ -84,6 +84,9 @@ def _router_grads(ctx, x, Wr, logits, idx, w, dw, dx):
     if ctx.num_experts % 64 == 0:
         dWr = G.grouped_gemm_wgrad(dlogits, x, seg, out_dtype=Wr.dtype)[0]            # [E, H]
     else:  # the token-major operand path tiles M in 64-wide atoms
+        if x.shape[0] % 8:   # transposed, the tokens are rows of whole 16-byte words
+            pad = (0, 0, 0, -x.shape[0] % 8)
+            dlogits, x = nn.functional.pad(dlogits, pad), nn.functional.pad(x, pad)
         dWr = G.grouped_gemm_wgrad(MO.transpose(dlogits), MO.transpose(x), seg, out_dtype=Wr.dtype, layout='mk')[0]
     return dx, dWr
 
