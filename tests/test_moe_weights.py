@@ -1,5 +1,4 @@
 """The quantised expert weights of a layer follow its weights, however those are written."""
-import os
 import socket
 
 import pytest
@@ -49,12 +48,13 @@ def _init_single():
     import torch.distributed as dist
     if dist.is_initialized():
         return
-    os.environ['MASTER_ADDR'] = '127.0.0.1'
+    # by address, not through the environment: other tests start children that would take the port from it
     with socket.socket() as s:
         s.bind(('127.0.0.1', 0))
-        os.environ['MASTER_PORT'] = str(s.getsockname()[1])
+        port = s.getsockname()[1]
     torch.cuda.set_device(0)
-    dist.init_process_group('nccl', rank=0, world_size=1, device_id=torch.device('cuda', 0))
+    dist.init_process_group('nccl', init_method=f'tcp://127.0.0.1:{port}', rank=0, world_size=1,
+                            device_id=torch.device('cuda', 0))
 
 
 def _buffer():
