@@ -20,6 +20,9 @@ __global__ void __launch_bounds__(256) quant_fp8_kernel(const T16* __restrict__ 
 
 void quant_fp8(const at::Tensor& x, at::Tensor q, at::Tensor scales, bool round_scale, double amax_floor) {
   const c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "x must be bf16 or fp16");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0,
+              "x must start on a 16-byte boundary, q on one of 8");
   TORCH_CHECK(x.is_contiguous() && q.is_contiguous() && scales.is_contiguous(), "contiguous tensors expected");
   const int H = static_cast<int>(x.size(-1));
   TORCH_CHECK(H % 128 == 0, "hidden must be a multiple of 128");
@@ -66,6 +69,8 @@ __global__ void __launch_bounds__(256) dequant_fp8_kernel(const uint8_t* __restr
 
 void dequant_fp8(const at::Tensor& q, const at::Tensor& scales, at::Tensor out) {
   const c10::cuda::CUDAGuard guard(q.device());
+  TORCH_CHECK(((reinterpret_cast<uintptr_t>(q.data_ptr()) | reinterpret_cast<uintptr_t>(out.data_ptr())) & 15) == 0,
+              "q and out must start on 16-byte boundaries");
   TORCH_CHECK(q.is_contiguous() && scales.is_contiguous() && out.is_contiguous(), "contiguous tensors expected");
   const int H = static_cast<int>(q.size(-1));
   TORCH_CHECK(H % 128 == 0 && q.element_size() == 1, "q must be e4m3 [.., H] with H % 128 == 0");

@@ -13,12 +13,19 @@ from ._ext import load
 GRAD_AMAX_FLOOR = 2.0 ** -116
 
 
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """Contiguous, on a 16-byte boundary (the kernels move 16 bytes at a time)."""
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
+
+
 def quantize_fp8(x: torch.Tensor, round_scale: bool = False, amax_floor: float = FP8_AMAX_FLOOR):
     """e4m3 with one fp32 scale ``max(amax, amax_floor) / 448`` per 128 channels (``round_scale``: its power-of-two
-    ceiling). Blocks far below the floor lose their values; gradients take ``GRAD_AMAX_FLOOR``."""
+    ceiling). Blocks far below the floor lose their values; gradients take ``GRAD_AMAX_FLOOR``. CUDA tensors are
+    bf16 or fp16."""
     if not x.is_cuda:
         return quantize_fp8_1x128(x, round_scale, amax_floor)
-    x = x.contiguous()
+    x = _aligned(x)
     H = x.shape[-1]
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     s = torch.empty(*x.shape[:-1], H // 128, dtype=torch.float32, device=x.device)
@@ -30,7 +37,7 @@ def dequantize_fp8(q: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """bf16 of e4m3 ``q`` [.., H] times its 1x128 fp32 ``scales`` [.., H/128] (one rounding)."""
     if not q.is_cuda:
         return dequantize_fp8_1x128(q, scales).to(torch.bfloat16)
-    q = q.contiguous()
+    q = _aligned(q)
     out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
     load().dequant_fp8(q.view(torch.uint8), scales.float().contiguous(), out)
     return out
