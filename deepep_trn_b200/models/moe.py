@@ -378,12 +378,20 @@ def reference_moe(x, Wr, W1, W2, topk, router_bias=None):
 
 
 def smoke_step(buf, dev):
-    """One tiny forward + backward of the layer (used by the build/smoke entry point)."""
+    """One tiny forward + backward of the layer (used by the build/smoke entry point), with the softmax gate in
+    bf16, and with the grouped gate and fp8 experts, whose generation step it runs too."""
     torch.manual_seed(0)
-    layer = MoELayer(buf, hidden=256, intermediate=256, num_experts=8 * buf.group_size, topk=2, device=dev)
+    E = 8 * buf.group_size
     x = (torch.randn(64, 256, device=dev) * 0.5).to(torch.bfloat16).requires_grad_()
-    y = layer(x)
-    y.float().square().mean().backward()
+    for kw in ({}, dict(gate=dict(scoring='sigmoid', num_groups=4, topk_groups=2, scale=2.5), fp8_block=True)):
+        layer = MoELayer(buf, hidden=256, intermediate=256, num_experts=E, topk=2, device=dev, **kw)
+        x.grad = None
+        y = layer(x)
+        y.float().square().mean().backward()
+        torch.cuda.synchronize()
+        assert torch.isfinite(y.float()).all() and torch.isfinite(x.grad.float()).all() and x.grad.abs().amax() > 0
+        assert layer.w1.grad is not None and torch.isfinite(layer.w1.grad.float()).all()
+    layer.quantize_weights()
+    out = layer.forward_low_latency(x.detach(), 64)
     torch.cuda.synchronize()
-    assert torch.isfinite(y.float()).all() and torch.isfinite(x.grad.float()).all()
-    assert layer.w1.grad is not None and torch.isfinite(layer.w1.grad.float()).all()
+    assert torch.isfinite(out.float()).all() and out.abs().amax() > 0
