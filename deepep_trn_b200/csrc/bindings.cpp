@@ -93,6 +93,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_gemm_fp8_m", &grouped_gemm_fp8_m);
   m.def("sf_tiles", &sf_tiles);
   m.def("grouped_gemm_fp8_block", &grouped_gemm_fp8_block);
+  m.def("error_word", &error_word);
   m.def("fp8_block_plan", &fp8_block_plan);
   m.def("quant_fp8_weight", &quant_fp8_weight);
   m.def("router_gate", &router_gate);

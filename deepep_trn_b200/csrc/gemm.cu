@@ -27,6 +27,7 @@
 // Every mbarrier wait is bounded; on timeout the CTA records an error, stops
 // issuing, lets the copies in flight land, frees its TMEM and returns.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include "ops.h"
 #include "tcgen05.cuh"
@@ -567,6 +568,22 @@ void launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc,
 }
 
 }  // namespace gemm
+
+// A zeroed int32 word of `device` that lives as long as the process. It is allocated and cleared apart from the
+// stream and the caching allocator: a word made inside a capture would lie in the graph's pool and hold
+// whatever was there until a replay clears it, and every replay would clear it again.
+at::Tensor error_word(int64_t device) {
+  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+  c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  void* p = nullptr;
+  cudaStream_t s = nullptr;
+  AT_CUDA_CHECK(cudaMalloc(&p, 256));
+  AT_CUDA_CHECK(cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking));
+  AT_CUDA_CHECK(cudaMemsetAsync(p, 0, 256, s));
+  AT_CUDA_CHECK(cudaStreamSynchronize(s));
+  AT_CUDA_CHECK(cudaStreamDestroy(s));
+  return at::from_blob(p, {1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+}
 
 // C[rows, N] = A[rows, K] @ B[g]^T per expert segment (offsets on rows, multiples of 128).
 // epilogue: 0 = bf16 C, 1 = fp32 C, 2 = SwiGLU (H = silu(gate) * up, C = pre-activation or none)

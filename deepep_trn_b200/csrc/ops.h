@@ -126,6 +126,8 @@ void grouped_gemm_fp8_m(const at::Tensor& A, const at::Tensor& sa, const at::Ten
 void grouped_gemm_k(const at::Tensor& A, const at::Tensor& B, const at::Tensor& offsets, at::Tensor C,
                     at::Tensor error, int64_t num_sms, double timeout_s, bool tok_major);
 
+at::Tensor error_word(int64_t device);
+
 // gemm_block.cu
 void grouped_gemm_fp8_block(const at::Tensor& A, const at::Tensor& sa, const at::Tensor& B, const at::Tensor& sb,
                             const OptTensor& offsets, const OptTensor& counts, const OptTensor& C, const OptTensor& H,

@@ -28,15 +28,15 @@ EPILOGUES = {'bf16': 0, 'f32': 1, 'swiglu': 2}
 
 
 def _err(dev) -> torch.Tensor:
-    key = (dev.type, dev.index)
+    index = torch.cuda.current_device() if dev.type == 'cuda' and dev.index is None else dev.index
+    key = (dev.type, index)
     if key not in _errors:
-        _errors[key] = torch.zeros(1, dtype=torch.int32, device=dev)
+        _errors[key] = load().error_word(index) if dev.type == 'cuda' else torch.zeros(1, dtype=torch.int32)
     return _errors[key]
 
 
 def check(device=None) -> None:
-    dev = device or torch.device('cuda', torch.cuda.current_device())
-    e = _err(dev)
+    e = _err(torch.device('cuda' if device is None else device))
     if int(e.item()):
         e.zero_()
         raise RuntimeError("a grouped GEMM or permute kernel gave up on a timed-out wait on the device")
