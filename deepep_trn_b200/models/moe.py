@@ -284,8 +284,9 @@ class MoELayer(nn.Module):
                                         for q, w in ((kept[0], self.w1), (kept[2], self.w2))):
             kept = None
         self._block_key = None
-        self._block_copy = (*G.quantize_fp8_weight(self.w1, out=kept and kept[:2]),
-                            *G.quantize_fp8_weight(self.w2, out=kept and kept[2:]))
+        with torch.inference_mode(False), torch.no_grad():   # (the copy is to be written outside of inference mode too)
+            self._block_copy = (*G.quantize_fp8_weight(self.w1, out=kept and kept[:2]),
+                                *G.quantize_fp8_weight(self.w2, out=kept and kept[2:]))
         self._block_key = self._weights_key()
 
     def _block_weights(self, train: bool):
