@@ -18,10 +18,13 @@
 // Forward and backward read each logit once (T * E) and write T * k * 12 or T * E; a warp takes
 // one token, its experts in the lanes' registers (16-byte loads and stores where the rows allow).
 // Values are compared as integers of the same order, so that one redux finds the warp's largest.
-// Bound by instruction issue (about 1000 a row of 256 experts, 8 groups, 8 chosen): 16384 such tokens
-// forward and backward in 37 us where their bytes would take 6 (59 us with values compared as floats by
-// shuffles, 4-byte accesses and ids looked for in every lane); one token 3.7 us (7.2 before), of which
-// 2.5 are a launch.
+// 16384 tokens of 256 experts, 8 groups, 8 chosen take 37 us forward and backward in a CUDA graph at 1965 MHz (43
+// as calls from the host) where their bytes would take 6; 59 us with values compared as floats by shuffles,
+// 4-byte accesses and ids looked for in every lane. One token takes 3.7 us in a graph, of which 2.5 are a launch
+// (7.2 before), and 5.8 as a call. What bounds them: forward half by instruction issue (1037 a row, 28.7 of
+// 59.6 thousand cycles), half by the chain of a row's dependent steps, which shows in the last wave of CTAs and
+// in rows that fp64 decides (an SM has work in 39 of the 59.6); backward by latency (269 a row, issue 40 % busy,
+// waiting for loads, exponentials and shared memory).
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>

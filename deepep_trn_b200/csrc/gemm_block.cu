@@ -22,15 +22,18 @@
 // fp32 scale per row and block (scale = max(amax, 1e-4) / 448), the operand of the next product.
 //
 // Two kernels, for groups with many and with few rows:
-//  * many: 128 rows x 256 columns, rows of A on the TMEM lanes; a CTA takes whole tiles. Bound by the
-//    operands' way into shared memory (48 KB a block at 64 bytes a cycle: 768 cycles).
-//    32 groups of 1024 rows, N 4096, K 7168, SwiGLU and pre-activation: 1180 us, 1630 TFLOP/s (1473 us
-//    with MMAs behind `lane == 0` and scales loaded by the threads that use them).
+//  * many: 128 rows x 256 columns, rows of A on the TMEM lanes; a CTA takes whole tiles. 32 groups of
+//    1024 rows, N 4096, K 7168, SwiGLU and pre-activation: 1205 us over a timed second, 1600 TFLOP/s, at
+//    1297 MHz, to which the 1000 W cap brings the clock: 28 rounds of 56 blocks, 1000 cycles a block. (1028 us
+//    in its first moments; 1473 us at about 1565 MHz and 1470 cycles with MMAs behind `lane == 0` and scales
+//    loaded by the threads that use them: a third of the cycles was a fifth of the time.) So energy a
+//    block bounds it as much as cycles a block, of which the operands' way into shared memory takes 768
+//    (48 KB at 64 bytes a cycle).
 //  * few (at most kFewTile rows): 256 columns x up to 48 rows, columns of C on the lanes, so that
 //    nothing is spent on rows that are not there. Bound by reading B: 32 slabs of 32 rows, the same N
-//    and K: 165 us, 5.8 TB/s (prefetching B into L2 ahead of the copies: 232 us). Tiles that do not fill
-//    a round of the SMs are taken by clusters that divide K and add their parts through distributed
-//    shared memory in a fixed order (one row, N 2048, K 7168: 10.5 us, 13.7 in the other form).
+//    and K: 152 us by itself, 6.2 TB/s (prefetching B into L2 ahead of the copies: 232 us). Tiles that do not
+//    fill a round of the SMs are taken by clusters that divide K and add their parts through distributed
+//    shared memory in a fixed order (4 rows, N 4096, K 4096: 11.5 us, 19.6 in the other form).
 // Segments take one of the two, by the rows that there are. For slabs, whose counts only the device
 // knows, both are launched where the second is worth it, and each takes its groups.
 //
@@ -76,8 +79,16 @@ enum BlkEpilogue : int { kOutBF16 = 0, kOutF32 = 1, kOutSwiGLU = 2 };
 
 // Estimated cycles, from measurements. A K block of a tile takes 900, or 1540 where all SMs read a part of
 // B of their own from memory. A tile with few rows costs 2300 more, and 6000 where a cluster divides K.
-// (Decoding, 32 groups of 32 rows: N 4096, K 7168, 512 tiles: 181 us as many rows, in 4 rounds, 165 as
-// few; N 7168, K 2048, 896 tiles: 88 and 98 us. One row, N 2048, K 7168: 13.7 and 10.5 us.)
+// How well they choose was measured with the form forced, for 1 to 64 groups of 4 to 200 rows, N 1408 to 7168,
+// K 512 to 7168:
+//  * 72 calls with segments: the form that is chosen takes at most 1.05 of the faster one's time in 66, and
+//    1.10 to 1.31 in 6, small calls with few groups (4 rows a group, N 2048, K 4096, 8 groups: 20.0 us as many
+//    rows, 16.1 as few);
+//  * 114 calls with slabs: at most 1.05 in 92. The second launch takes 5 to 8 us that are not in the estimates,
+//    wherever both are launched: 32 slabs of 32 rows, N 4096, K 7168: 162 us as many rows, 152 as few, 168
+//    with both; the worst is one slab of 4 rows, N 4096, K 4096: 20.1, 11.7 and 19.4. The groups divided
+//    between the two were not the faster way in any call (13 slabs of 2 to 126 rows, N 3584, K 6656: 71 us as
+//    many rows, 78 as few, 82 divided).
 __host__ __device__ inline int64_t block_cycles(int64_t ctas, int64_t sms, bool own) { return own && ctas * 2 > sms ? 1540 : 900; }
 __host__ __device__ inline int64_t many_cycles(int64_t tiles, int64_t KB, int64_t sms, bool own) {
   return (tiles + sms - 1) / sms * KB * block_cycles(tiles, sms, own) + 4000;
