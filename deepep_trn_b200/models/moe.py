@@ -274,11 +274,16 @@ class MoELayer(nn.Module):
         the replays of a captured step see the new weights from then on. Calls on other streams are ordered
         behind it as behind any write to the weights. The copy is left aside once the weights' version or
         address differs, and after a call with gradients, which an update follows; only a write through
-        ``w.data`` outside of training goes unseen."""
-        if not self.fp8_block:
-            raise ValueError('quantize_weights needs fp8_block=True')
+        ``w.data`` outside of training goes unseen. An ``fp8_experts`` layer, which keeps a copy by itself, makes
+        that one anew."""
+        if not (self.fp8_block or self.fp8_experts):
+            raise ValueError('quantize_weights needs fp8_block=True or fp8_experts=True')
         if self.w1.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError('quantize_weights must be called outside of a capture')
+        if self.fp8_experts:
+            self._fp8_cache = None
+            self._fp8_weights()
+            return
         kept = self._block_copy
         if kept is not None and not all(q.shape == w.shape and q.device == w.device
                                         for q, w in ((kept[0], self.w1), (kept[2], self.w2))):
