@@ -270,12 +270,15 @@ class MoELayer(nn.Module):
     def quantize_weights(self) -> None:
         """Quantises the expert weights of an ``fp8_block`` layer into a copy that ``forward_low_latency`` and
         calls without gradients then read instead of quantising the weights themselves (0.67 ms for 32
-        experts, W1 4096 x 7168 and W2 7168 x 2048). Call it again after a change of the weights: it writes into the same storage, so
-        the replays of a captured step see the new weights from then on. Calls on other streams are ordered
-        behind it as behind any write to the weights. The copy is left aside once the weights' version or
-        address differs, and after a call with gradients, which an update follows; what leaves no trace in
-        Python (a write through ``w.data`` outside of training, a replayed optimizer step) goes unseen. An ``fp8_experts`` layer, which keeps a copy by itself, makes
-        that one anew."""
+        experts, W1 4096 x 7168 and W2 7168 x 2048).
+
+        Call it again after a change of the weights: it writes into the same storage, so the replays of a
+        captured step see the new weights from then on. Calls on other streams are ordered behind it as behind
+        any write to the weights. The copy is left aside once the weights' version or address differs, and
+        after a call with gradients, which an update follows. What leaves no trace in Python (a write through
+        ``w.data`` outside of training, a replayed optimizer step) goes unseen.
+
+        An ``fp8_experts`` layer, which keeps a copy by itself, makes that one anew."""
         if not (self.fp8_block or self.fp8_experts):
             raise ValueError('quantize_weights needs fp8_block=True or fp8_experts=True')
         if self.w1.is_cuda and torch.cuda.is_current_stream_capturing():
